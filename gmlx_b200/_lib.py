@@ -27,8 +27,16 @@ class ChainProblem(ctypes.Structure):
 
 KQ_CHAIN_MAX = 8
 
+
+class PagedCache(ctypes.Structure):
+    """struct kq_paged_cache (include/kq_cuda.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int), ("pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("kv_heads", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("page_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
 # Every symbol include/kq_cuda.h declares, with its ctypes signature.
-_vp, _i32, _i64, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t
+_vp, _i32, _i64, _sz, _f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_size_t, ctypes.c_float
 SIGNATURES = {
     "kq_version": (_i32, []),
     "kq_last_error": (ctypes.c_char_p, []),
@@ -72,6 +80,14 @@ SIGNATURES = {
     "kq_ipc_handle": (_i32, [_vp, _vp]),
     "kq_ipc_open": (_i32, [_vp, _vp]),
     "kq_ipc_close": (_i32, [_vp]),
+    "kq_paged_plan": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                             _vp]),
+    "kq_rope_kv_write": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i32,
+                                _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "kq_paged_attention": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i64, _i64, _f32, _i32,
+                                  _i64, _f32, _vp, _vp, _vp, _sz, _vp]),
+    "kq_paged_attention_workspace_size": (_sz, [_i64]),
+    "kq_moe_route": (_i32, [_vp, _i32, _i64, _i64, _i64, _i32, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _vp, _vp]),
 }
 
 _lib = None

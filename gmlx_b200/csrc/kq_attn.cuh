@@ -1,0 +1,88 @@
+// kq_attn.cuh -- what the two attention kernels share: the geometry of a
+// request, the split of the work over the grid, and the join of split rows.
+//
+// A request with n new tokens of L in all is n * G packed rows for each of its
+// kv heads (row r is token r / G, query head h * G + r % G), so the query heads
+// that share a kv head read its keys once.  Row r sees the keys
+// [limit - window, limit), limit = L - n + r / G + 1.
+#pragma once
+#include <math.h>
+
+#include "kq_ptx.cuh"
+#include "kq_serve.cuh"
+
+namespace kq {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Request {
+    int q0, n, len;
+};
+
+// Request b of the call; b == B stands for the padding tokens behind the last
+// one (no keys: their rows are written as empty).  Lengths that contradict the
+// buffers are cut to them and reported.
+__device__ __forceinline__ Request load_request(const AttnArgs &a, int b, bool &bad) {
+    Request r;
+    const int c0 = a.cu[b], c1 = b < a.B ? a.cu[b + 1] : a.T;
+    const int s = b < a.B ? a.seq[b] : 0;
+    r.q0 = min(max(c0, 0), a.T);
+    const int e = min(max(c1, r.q0), a.T);
+    r.n = e - r.q0;
+    r.len = min(max(s, 0), a.max_len);
+    bad |= r.q0 != c0 || e != c1 || r.len != s;
+    return r;
+}
+
+// Keys [lo, hi) that the rows of tokens [t0, t1) of a request can see.
+__device__ __forceinline__ void key_range(const AttnArgs &a, const Request &r, int t0, int t1, int &lo, int &hi) {
+    hi = a.causal ? max(0, r.len - r.n + t1) : r.len;
+    lo = a.window ? max(0, r.len - r.n + t0 + 1 - a.window) : 0;
+    lo = min(lo, hi);
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// cap * tanh(z / cap) in units of log2, from one exponential and one reciprocal:
+// tanh(u) = 1 - 2 / (1 + e^2u) (the hardware's tanh is good to 11 bits only,
+// too few for a score of up to `cap`)
+__device__ __forceinline__ float soft_cap(float x, float in2, float out) {
+    return out - __fdividef(2.0f * out, 1.0f + ex2(x * in2));
+}
+
+// Unit u of `total` belongs to block ((u + 1) * grid - 1) / total, when block c
+// takes the units [c * total / grid, (c + 1) * total / grid).
+__device__ __forceinline__ int64_t unit_begin(int64_t total, int c, int grid) { return total * c / grid; }
+__device__ __forceinline__ int unit_block(int64_t total, int64_t u, int grid) { return (int)(((u + 1) * grid - 1) / total); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool full) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldsm4(uint32_t r[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t r[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+template <bool F16> __device__ __forceinline__ uint32_t pack_half(float x, float y) {
+    uint32_t v;
+    if (F16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(y), "f"(x));
+    return v;
+}
+
+}  // namespace kq

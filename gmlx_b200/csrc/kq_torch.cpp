@@ -1,4 +1,5 @@
-// kq_torch.cpp -- native fast path of the decode-time kq ops for torch tensors.
+// kq_torch.cpp -- native fast path of the decode-time kq ops for torch tensors
+// (the projections and the operators of the serving step around them).
 //
 // kq.quantized_matmul / kq.quantized_glu are called once per projection per
 // token; going through Python argument handling and ctypes costs ~15-20 us a
@@ -17,12 +18,15 @@
 // uses too (workspace()), so kq.workspace_error() sees every call's error word.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <cstdint>
 #include <map>
 #include <mutex>
 #include <tuple>
+
+#include "../../include/kq_cuda.h"
 
 namespace {
 
@@ -156,6 +160,136 @@ py::object quantized_glu(const at::Tensor &x, const at::Tensor &wg, const at::Te
     return py::cast(shaped(y, x, n));
 }
 
+// ---- the serving step ------------------------------------------------------
+// As above: each takes the well-formed call and returns None for the rest.
+
+decltype(&kq_paged_plan) g_plan = nullptr;
+decltype(&kq_rope_kv_write) g_rope = nullptr;
+decltype(&kq_paged_attention) g_attn = nullptr;
+decltype(&kq_paged_attention_workspace_size) g_attn_ws = nullptr;
+decltype(&kq_moe_route) g_route = nullptr;
+
+void set_serve_entry_points(int64_t plan, int64_t rope, int64_t attn, int64_t attn_ws, int64_t route) {
+    g_plan = reinterpret_cast<decltype(g_plan)>(plan);
+    g_rope = reinterpret_cast<decltype(g_rope)>(rope);
+    g_attn = reinterpret_cast<decltype(g_attn)>(attn);
+    g_attn_ws = reinterpret_cast<decltype(g_attn_ws)>(attn_ws);
+    g_route = reinterpret_cast<decltype(g_route)>(route);
+}
+
+bool vec(const at::Tensor &t, int64_t n, at::ScalarType type, int dev) {
+    return t.is_cuda() && t.get_device() == dev && t.dim() == 1 && (n < 0 || t.size(0) == n) && t.scalar_type() == type &&
+           t.is_contiguous();
+}
+
+int64_t st(const at::Tensor &t, int i) { return t.size(i) == 1 ? 0 : t.stride(i); }
+bool dense(const at::Tensor &t, int i) { return t.size(i) <= 1 || t.stride(i) == 1; }
+
+bool table_ok(const at::Tensor &t, int64_t b, int dev) {
+    return t.is_cuda() && t.get_device() == dev && t.dim() == 2 && t.size(0) == b && t.scalar_type() == at::kInt &&
+           dense(t, 1);
+}
+int64_t table_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+bool cache_of(const at::Tensor &k, const at::Tensor &v, kq_paged_cache &c) {
+    if (!k.is_cuda() || !v.is_cuda() || v.get_device() != k.get_device() || k.dim() != 4 || v.dim() != 4 ||
+        k.sizes() != v.sizes() || k.scalar_type() != v.scalar_type() || k.numel() == 0)
+        return false;
+    const int code = dtype_code(k.scalar_type());
+    if (code < 1) return false;
+    for (int i = 0; i < 4; i++)
+        if (st(k, i) != st(v, i)) return false;
+    if (!dense(k, 3)) return false;
+    c = kq_paged_cache{k.data_ptr(), v.data_ptr(), code, k.size(0), k.size(1), k.size(2), k.size(3), st(k, 0), st(k, 1), st(k, 2)};
+    return true;
+}
+
+bool heads_ok(const at::Tensor &t, const kq_paged_cache &c, int dev) {
+    return t.is_cuda() && t.get_device() == dev && t.dim() == 3 && t.size(2) == c.dim && dtype_code(t.scalar_type()) == c.dtype &&
+           dense(t, 2) && st(t, 0) % 8 == 0 && st(t, 1) % 8 == 0 && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
+}
+
+at::Tensor stream_workspace(int dev, cudaStream_t s, size_t bytes) { return workspace(dev, reinterpret_cast<int64_t>(s), (int64_t)bytes); }
+
+py::object paged_plan(const at::Tensor &ctx, const at::Tensor &qlen, const at::Tensor &table, const at::Tensor &free_pages,
+                      int64_t page, int64_t tokens) {
+    if (!g_plan || !ctx.is_cuda() || tokens < 0) return py::none();
+    const int dev = ctx.get_device();
+    if (!vec(ctx, -1, at::kInt, dev)) return py::none();
+    const int64_t b = ctx.size(0);
+    if (!vec(qlen, b, at::kInt, dev) || !vec(free_pages, -1, at::kInt, dev) || !table_ok(table, b, dev)) return py::none();
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    const auto i32 = ctx.options();
+    at::Tensor cu = at::empty({b + 1}, i32), seq = at::empty({b}, i32), slots = at::empty({tokens}, i32.dtype(at::kLong)),
+               pos = at::empty({tokens}, i32), used = at::empty({1}, i32);
+    cudaStream_t s = at::cuda::getCurrentCUDAStream(dev).stream();
+    at::Tensor ws = stream_workspace(dev, s, 256);
+    const int rc = g_plan(ctx.data_ptr<int>(), qlen.data_ptr<int>(), b, table.data_ptr<int>(), table_stride(table), table.size(1),
+                          free_pages.data_ptr<int>(), free_pages.size(0), page, tokens, cu.data_ptr<int>(), seq.data_ptr<int>(),
+                          slots.data_ptr<int64_t>(), pos.data_ptr<int>(), used.data_ptr<int>(), ws.data_ptr(), (size_t)ws.numel(), s);
+    if (rc) return py::none();
+    return py::make_tuple(cu, seq, slots, pos, used);
+}
+
+py::object rope_kv_write(const at::Tensor &q, const at::Tensor &k, const at::Tensor &v, const at::Tensor &cos, const at::Tensor &sin,
+                         const at::Tensor &pos, const at::Tensor &kc, const at::Tensor &vc, const at::Tensor &slots, bool interleaved) {
+    kq_paged_cache c;
+    if (!g_rope || !cache_of(kc, vc, c)) return py::none();
+    const int dev = kc.get_device();
+    if (!heads_ok(q, c, dev) || !heads_ok(k, c, dev) || !heads_ok(v, c, dev)) return py::none();
+    const int64_t t = q.size(0), h = q.size(1);
+    if (k.size(0) != t || v.size(0) != t || k.size(1) != c.kv_heads || v.size(1) != c.kv_heads) return py::none();
+    if (!cos.is_cuda() || cos.get_device() != dev || cos.dim() != 2 || cos.scalar_type() != at::kFloat || !cos.is_contiguous() ||
+        !sin.is_cuda() || sin.get_device() != dev || sin.sizes() != cos.sizes() || sin.scalar_type() != at::kFloat || !sin.is_contiguous())
+        return py::none();
+    if (!vec(pos, t, at::kInt, dev) || !vec(slots, t, at::kLong, dev)) return py::none();
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    at::Tensor out = at::empty({t, h, c.dim}, q.options());
+    cudaStream_t s = at::cuda::getCurrentCUDAStream(dev).stream();
+    at::Tensor ws = stream_workspace(dev, s, 256);
+    const int rc = g_rope(&c, q.data_ptr(), st(q, 0), st(q, 1), k.data_ptr(), st(k, 0), st(k, 1), v.data_ptr(), st(v, 0), st(v, 1), t,
+                          h, cos.data_ptr<float>(), sin.data_ptr<float>(), cos.size(0), (int)(2 * cos.size(1)), interleaved,
+                          pos.data_ptr<int>(), slots.data_ptr<int64_t>(), out.data_ptr(), ws.data_ptr(), (size_t)ws.numel(), s);
+    if (rc) return py::none();
+    return py::cast(out);
+}
+
+py::object paged_attention(const at::Tensor &q, const at::Tensor &kc, const at::Tensor &vc, const at::Tensor &table, const at::Tensor &seq,
+                           const at::Tensor &cu, int64_t max_query_len, double scale, int64_t window, double softcap, bool causal,
+                           bool return_lse) {
+    kq_paged_cache c;
+    if (!g_attn || !cache_of(kc, vc, c)) return py::none();
+    const int dev = kc.get_device();
+    if (!heads_ok(q, c, dev) || !vec(seq, -1, at::kInt, dev)) return py::none();
+    const int64_t t = q.size(0), h = q.size(1), b = seq.size(0);
+    if (!vec(cu, b + 1, at::kInt, dev) || !table_ok(table, b, dev)) return py::none();
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    at::Tensor out = at::empty({t, h, c.dim}, q.options()), lse;
+    if (return_lse) lse = at::empty({t, h}, q.options().dtype(at::kFloat));
+    cudaStream_t s = at::cuda::getCurrentCUDAStream(dev).stream();
+    at::Tensor ws = stream_workspace(dev, s, g_attn_ws(c.dim));
+    const int rc = g_attn(&c, q.data_ptr(), st(q, 0), st(q, 1), t, h, table.data_ptr<int>(), table_stride(table), table.size(1),
+                          seq.data_ptr<int>(), cu.data_ptr<int>(), b, max_query_len, (float)scale, causal, window, (float)softcap,
+                          out.data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), (size_t)ws.numel(), s);
+    if (rc) return py::none();
+    return return_lse ? py::object(py::make_tuple(out, lse)) : py::object(py::cast(out));
+}
+
+py::object moe_route(const at::Tensor &logits, int64_t k, int64_t scoring, const c10::optional<at::Tensor> &bias, int64_t n_groups,
+                     int64_t topk_groups, bool norm, double scale) {
+    if (!g_route || !logits.is_cuda() || logits.dim() != 2 || k < 1) return py::none();
+    const int code = dtype_code(logits.scalar_type()), dev = logits.get_device();
+    const int64_t t = logits.size(0), e = logits.size(1);
+    if (code < 0 || !dense(logits, 1) || (bias && !vec(*bias, e, at::kFloat, dev))) return py::none();
+    c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+    at::Tensor idx = at::empty({t, k}, logits.options().dtype(at::kInt)), w = at::empty({t, k}, logits.options().dtype(at::kFloat));
+    cudaStream_t s = at::cuda::getCurrentCUDAStream(dev).stream();
+    const int rc = g_route(logits.data_ptr(), code, t, e, st(logits, 0), (int)k, (int)scoring, bias ? bias->data_ptr<float>() : nullptr,
+                           (int)n_groups, (int)topk_groups, norm, (float)scale, idx.data_ptr<int>(), w.data_ptr<float>(), s);
+    if (rc) return py::none();
+    return py::make_tuple(idx, w);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -164,4 +298,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("workspace_peek", &workspace_peek);
     m.def("quantized_matmul", &quantized_matmul);
     m.def("quantized_glu", &quantized_glu);
+    m.def("set_serve_entry_points", &set_serve_entry_points);
+    m.def("paged_plan", &paged_plan);
+    m.def("rope_kv_write", &rope_kv_write);
+    m.def("paged_attention", &paged_attention);
+    m.def("moe_route", &moe_route);
 }

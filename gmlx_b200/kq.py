@@ -21,6 +21,12 @@ kq op                      gmlx call sites
 ``codec_has_matmul``       (modules.py:155-234)
 =========================  =============================================
 
+Four more operators make a serving step of the projections above:
+``paged_plan`` (block tables, slots and positions from request lengths),
+``rope_kv_write`` (rotary embedding, keys and values into a paged cache),
+``paged_attention`` (the new tokens over their requests' pages) and
+``moe_route`` (softmax or sigmoid scores, balance bias, groups, top-k).
+
 Weights are uint8 wire-byte tensors ``[N, K/256*bpb]`` (or ``[E, N, ...]``),
 never repacked; ``scales`` is the reference's ``(1,)`` placeholder and is
 ignored.  Outputs are fresh tensors in the activation dtype.  Unknown codecs
@@ -30,6 +36,8 @@ on the current torch CUDA stream.
 from __future__ import annotations
 
 import ctypes as _ct
+import math
+from typing import NamedTuple
 
 import torch
 
@@ -40,6 +48,7 @@ __all__ = [
     "codecs", "all_codecs", "codec_has_matmul", "codec_has_moe_glu", "block_bytes", "dequantize", "quantized_matmul", "quantized_glu", "gather_qmm",
     "moe_glu_gather_kq", "gather_qmv_kq", "gather_qmv_mix_ns_kq", "moe_router_topk", "workspace_error",
     "moe_expert_layer_local", "quantized_matmul_chain", "quantized_matmul_allreduce", "quantized_matmul_qmv_bias", "moe_glu_gather_shexp_kq", "gather_qmv_mix_kq",
+    "PagedPlan", "paged_plan", "rope_kv_write", "paged_attention", "moe_route",
 ]
 
 _DT = {torch.float32: _lib.KQ_F32, torch.float16: _lib.KQ_F16, torch.bfloat16: _lib.KQ_BF16}
@@ -173,6 +182,8 @@ def _ext():
             addr = lambda f: _ct.cast(f, _ct.c_void_p).value  # noqa: E731
             e.set_entry_points(addr(L.kq_quantized_matmul), addr(L.kq_quantized_glu),
                                addr(L.kq_quantized_matmul_workspace_size), addr(L.kq_quantized_glu_workspace_size))
+            e.set_serve_entry_points(addr(L.kq_paged_plan), addr(L.kq_rope_kv_write), addr(L.kq_paged_attention),
+                                     addr(L.kq_paged_attention_workspace_size), addr(L.kq_moe_route))
         _EXT = e if e is not None else False
     return _EXT or None
 
@@ -693,3 +704,261 @@ def quantized_matmul_chain(problems, out_dtype: torch.dtype | None = None) -> li
     _lib.check(L.kq_quantized_matmul_chain(arr, n, _DT[x_dtype], _p(ws), ws.numel(), _stream(dev)),
                "quantized_matmul_chain")
     return outs
+
+
+# --------------------------------------------------------------------------
+# the serving step around the projections
+
+
+class PagedPlan(NamedTuple):
+    """What ``paged_plan`` gives: row offsets of the requests' new tokens
+    ``[batch + 1]``, lengths with the new tokens ``[batch]`` (both int32), cache
+    slots (int64) and positions (int32) of the tokens, pages taken ``[1]`` (int32)."""
+    cu_seqlens: torch.Tensor
+    seq_lens: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    pages_used: torch.Tensor
+
+
+def _same_device(what: str, *ts):
+    _need_cuda(*ts)
+    dev = next(t for t in ts if t is not None).device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _vector(what: str, name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> torch.Tensor:
+    if t.dim() != 1 or (n >= 0 and t.shape[0] != n) or t.dtype != dtype:
+        raise ValueError(f"{what}: {name} must be a {dtype} vector{f' of {n}' if n >= 0 else ''}, "
+                         f"got {t.dtype} {tuple(t.shape)}")
+    return t.contiguous()
+
+
+def _table(what: str, t: torch.Tensor, batch: int) -> tuple[int, int]:
+    """(row stride, width) of int32 block tables."""
+    if t.dim() != 2 or t.shape[0] != batch or t.dtype != torch.int32:
+        raise ValueError(f"{what}: block_tables must be int32 [{batch}, pages], got {t.dtype} {tuple(t.shape)}")
+    if not _dense_last(t):
+        raise ValueError(f"{what}: block_tables rows must be contiguous")
+    w = t.shape[1]
+    return (t.stride(0) if batch > 1 else w), w
+
+
+def _strides(t: torch.Tensor) -> list[int]:
+    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
+
+
+def _dense_last(t: torch.Tensor) -> bool:
+    return t.shape[-1] <= 1 or t.stride(-1) == 1
+
+
+def _paged_cache(what: str, k: torch.Tensor, v: torch.Tensor) -> "_lib.PagedCache":
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
+        raise ValueError(f"{what}: the caches must be [pages, page_size, kv_heads, dim] of one shape and type, "
+                         f"got {k.dtype} {tuple(k.shape)} and {v.dtype} {tuple(v.shape)}")
+    if k.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"{what}: the caches must be bf16 or fp16, got {k.dtype}")
+    if 0 in k.shape:
+        raise ValueError(f"{what}: an empty cache {tuple(k.shape)}")
+    s = _strides(k)
+    if s != _strides(v) or not _dense_last(k):
+        raise ValueError(f"{what}: the caches must share their strides, with contiguous heads")
+    return _lib.PagedCache(_p(k), _p(v), _DT[k.dtype], *k.shape, *s[:3])
+
+
+def _heads(what: str, name: str, t: torch.Tensor, dim: int, dtype: torch.dtype) -> torch.Tensor:
+    """[tokens, heads, dim] with contiguous, 16-byte aligned heads (copied if they are not)."""
+    if t.dim() != 3 or t.shape[2] != dim or t.dtype != dtype:
+        raise ValueError(f"{what}: {name} must be {dtype} [tokens, heads, {dim}], got {t.dtype} {tuple(t.shape)}")
+    s = _strides(t)
+    if not _dense_last(t) or s[0] % 8 or s[1] % 8 or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def paged_plan(context_lens: torch.Tensor, query_lens: torch.Tensor, block_tables: torch.Tensor,
+               free_pages: torch.Tensor, page_size: int, num_tokens: int) -> PagedPlan:
+    """Block tables and slot map of a step, built on the GPU from the requests'
+    lengths in one launch: request ``b`` has ``context_lens[b]`` tokens cached
+    and ``query_lens[b]`` new ones (int32 vectors, up to 8192 requests).  The
+    pages it lacks come from ``free_pages`` (int32, handed out from its front in
+    request order) and are written into its row of ``block_tables`` (int32
+    ``[batch, pages]``, in place); token ``i`` of the request stands at position
+    ``context + i``, in slot ``page * page_size + position % page_size``.
+
+    ``num_tokens`` is the length of the step's token buffers: tokens past the
+    last request are padding (slot -1, position 0).  Lengths that do not fit the
+    buffers (negative, more tokens than ``num_tokens``) set the workspace error
+    20, a missing page (``free_pages`` or the table's row too short) gives slot
+    -1 and error 21; ``pages_used`` counts the pages that were needed."""
+    b = context_lens.shape[0] if context_lens.dim() == 1 else -1
+    e = _ext()
+    if e is not None:  # native fast path; None: the full path below (and its errors)
+        r = e.paged_plan(context_lens, query_lens, block_tables, free_pages, page_size, num_tokens)
+        if r is not None:
+            return PagedPlan(*r)
+    dev = _same_device("paged_plan", context_lens, query_lens, block_tables, free_pages)
+    ctx = _vector("paged_plan", "context_lens", context_lens, -1, torch.int32)
+    new = _vector("paged_plan", "query_lens", query_lens, b, torch.int32)
+    free = _vector("paged_plan", "free_pages", free_pages, -1, torch.int32)
+    stride, width = _table("paged_plan", block_tables, b)
+    i32 = dict(dtype=torch.int32, device=dev)
+    if num_tokens < 0:
+        raise ValueError(f"paged_plan: num_tokens = {num_tokens}")
+    out = PagedPlan(torch.empty(b + 1, **i32), torch.empty(b, **i32),
+                    torch.empty(num_tokens, dtype=torch.int64, device=dev), torch.empty(num_tokens, **i32),
+                    torch.empty(1, **i32))
+    with torch.cuda.device(dev):
+        ws = _workspace(dev, 256)
+        _lib.check(_lib.load().kq_paged_plan(_p(ctx), _p(new), b, _p(block_tables), stride, width, _p(free),
+                                             free.shape[0], page_size, num_tokens, _p(out.cu_seqlens),
+                                             _p(out.seq_lens), _p(out.slots), _p(out.positions), _p(out.pages_used),
+                                             _p(ws), ws.numel(), _stream(dev)), "paged_plan")
+    return out
+
+
+def rope_kv_write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
+                  positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor,
+                  interleaved: bool = False) -> torch.Tensor:
+    """Rotary embedding of a step's queries and keys, and the store of its keys
+    and values into the paged cache, in one launch; returns the turned queries.
+
+    ``q [tokens, heads, dim]``, ``k``, ``v [tokens, kv_heads, dim]`` may be views
+    of one fused projection; ``cos``, ``sin`` are f32 ``[positions, rot / 2]``:
+    the first ``rot`` values of each head turn by their token's row, in pairs
+    ``(2i, 2i + 1)`` when ``interleaved``, else ``(i, i + rot / 2)``, in f32 with
+    one rounding at the end; ``dim`` and ``rot`` are multiples of 16.
+    ``positions`` (int32) and ``slots`` (int64) are per token, as ``paged_plan``
+    gives them; a token with a negative slot is not stored.  The caches are
+    ``[pages, page_size, kv_heads, dim]``.  A position outside the angle table is
+    cut to it and a slot outside the cache skipped, with workspace error 22."""
+    e = _ext()
+    if e is not None:  # native fast path; None: the full path below (and its errors)
+        r = e.rope_kv_write(q, k, v, cos, sin, positions, k_cache, v_cache, slots, interleaved)
+        if r is not None:
+            return r
+    what = "rope_kv_write"
+    dev = _same_device(what, q, k, v, cos, sin, positions, k_cache, v_cache, slots)
+    cache = _paged_cache(what, k_cache, v_cache)
+    dim, hk = cache.dim, cache.kv_heads
+    q, k, v = (_heads(what, n, t, dim, k_cache.dtype) for n, t in (("q", q), ("k", k), ("v", v)))
+    t, hq = q.shape[:2]
+    if k.shape[:2] != (t, hk) or v.shape[:2] != (t, hk):
+        raise ValueError(f"{what}: k and v must be [{t}, {hk}, {dim}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise ValueError(f"{what}: cos and sin must be f32 [positions, rot / 2] of one shape")
+    cos, sin = cos.contiguous(), sin.contiguous()
+    pos = _vector(what, "positions", positions, t, torch.int32)
+    slot = _vector(what, "slots", slots, t, torch.int64)
+    out = torch.empty(t, hq, dim, dtype=q.dtype, device=dev)
+    with torch.cuda.device(dev):
+        ws = _workspace(dev, 256)
+        qs, ks, vs = _strides(q), _strides(k), _strides(v)
+        _lib.check(_lib.load().kq_rope_kv_write(_ct.byref(cache), _p(q), qs[0], qs[1], _p(k), ks[0], ks[1], _p(v),
+                                                vs[0], vs[1], t, hq, _p(cos), _p(sin), cos.shape[0], 2 * cos.shape[1],
+                                                int(bool(interleaved)), _p(pos), _p(slot), _p(out), _p(ws), ws.numel(),
+                                                _stream(dev)), what)
+    return out
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                    seq_lens: torch.Tensor, cu_seqlens: torch.Tensor, max_query_len: int, scale: float | None = None,
+                    window: int = 0, softcap: float = 0.0, causal: bool = True, return_lse: bool = False):
+    """Attention of each request's new tokens over its pages of the cache.
+
+    ``q [tokens, heads, dim]`` (dim 64, 128 or 256) holds the new tokens of all
+    requests, those of request ``b`` in rows ``cu_seqlens[b] .. cu_seqlens[b+1]``
+    (int32); its keys and values are the first ``seq_lens[b]`` (int32, the new
+    tokens among them) rows of the pages in ``block_tables[b]``; the caches are
+    ``[pages, page_size, kv_heads, dim]`` and each kv head serves
+    ``heads / kv_heads`` query heads in a row.  Row ``i`` of ``n`` sees the keys
+    below ``seq_len - n + i + 1`` (all of the request's when not ``causal``), and
+    only the last ``window`` of those when ``window > 0``.  Scores are
+    ``scale * q.k`` (default ``dim ** -0.5``), capped as
+    ``softcap * tanh(score / softcap)`` when ``softcap > 0``; scores, maxima and
+    sums are held in f32.  Returns ``out`` like ``q``, with ``return_lse`` also
+    the log of each row's sum, f32 ``[tokens, heads]``.
+
+    A row that sees no key, and tokens past the last request, give 0 and -inf.
+    What the cache holds past a request's length, or before every row's window,
+    is never used, whatever bytes it has; the values a request does have must be
+    finite.  ``max_query_len`` only picks the kernels.  Lengths that contradict
+    the buffers are cut to them (workspace error 20); a page id outside the cache
+    counts as a page of zeros (error 22)."""
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    e = _ext()
+    if e is not None:  # native fast path; None: the full path below (and its errors)
+        r = e.paged_attention(q, k_cache, v_cache, block_tables, seq_lens, cu_seqlens, max_query_len, scale, window,
+                              softcap, causal, return_lse)
+        if r is not None:
+            return r
+    what = "paged_attention"
+    dev = _same_device(what, q, k_cache, v_cache, block_tables, seq_lens, cu_seqlens)
+    cache = _paged_cache(what, k_cache, v_cache)
+    q = _heads(what, "q", q, cache.dim, k_cache.dtype)
+    t, hq = q.shape[:2]
+    seq = _vector(what, "seq_lens", seq_lens, -1, torch.int32)
+    b = seq.shape[0]
+    cu = _vector(what, "cu_seqlens", cu_seqlens, b + 1, torch.int32)
+    stride, width = _table(what, block_tables, b)
+    if not math.isfinite(scale) or not math.isfinite(softcap):
+        raise ValueError(f"{what}: scale {scale}, softcap {softcap}")
+    out = torch.empty(t, hq, cache.dim, dtype=q.dtype, device=dev)
+    lse = torch.empty(t, hq, dtype=torch.float32, device=dev) if return_lse else None
+    with torch.cuda.device(dev):
+        ws = _workspace(dev, _ws_size("kq_paged_attention_workspace_size", cache.dim))
+        qs = _strides(q)
+        _lib.check(_lib.load().kq_paged_attention(_ct.byref(cache), _p(q), qs[0], qs[1], t, hq, _p(block_tables),
+                                                  stride, width, _p(seq), _p(cu), b, max_query_len, scale,
+                                                  int(bool(causal)), window, softcap, _p(out), _p(lse), _p(ws),
+                                                  ws.numel(), _stream(dev)), what)
+    return (out, lse) if return_lse else out
+
+
+_SCORES = {"softmax": 0, "sigmoid": 1}
+
+
+def moe_route(logits: torch.Tensor, k: int, scoring: str = "softmax", bias: torch.Tensor | None = None,
+              n_groups: int = 1, topk_groups: int = 1, norm_topk_prob: bool = True, scale: float = 1.0):
+    """Experts and weights of each token: scores are the softmax or sigmoid of
+    ``logits [..., experts]`` (f32, bf16 or fp16; up to 1024 experts), the choice
+    of ``k`` (up to 32) goes by score + ``bias`` (f32 ``[experts]``, the balance
+    bias), and with ``n_groups > 1`` only among the ``topk_groups`` groups of
+    consecutive experts whose two best sum highest.  Returns int32 indices and
+    f32 weights ``[..., k]``: descending by the choice, ties to the lower index;
+    the weights are the scores without bias, divided by their sum when
+    ``norm_topk_prob``, times ``scale``.
+
+    ``moe_router_topk`` is the reference's softmax router with a shared gate; this
+    one adds what DeepSeek-V3-like layers need.  A NaN logit counts as -inf (a
+    masked expert); a row whose chosen scores are all 0 gets weights 0."""
+    if scoring not in _SCORES:
+        raise ValueError(f"moe_route: scoring must be one of {sorted(_SCORES)}, got {scoring!r}")
+    e_ = _ext()
+    if e_ is not None:  # native fast path; None: the full path below (and its errors)
+        r = e_.moe_route(logits, k, _SCORES[scoring], bias, n_groups, topk_groups, norm_topk_prob, scale)
+        if r is not None:
+            return r
+    dev = _same_device("moe_route", logits, bias)
+    if logits.dim() < 1 or logits.dtype not in _DT:
+        raise ValueError(f"moe_route: logits must be f32, bf16 or fp16 [..., experts], got {logits.dtype}")
+    e = logits.shape[-1]
+    lg = logits.reshape(-1, e) if e else logits.reshape(0, 0)
+    if not _dense_last(lg):
+        lg = lg.contiguous()
+    t = lg.shape[0]
+    if bias is not None:
+        bias = _vector("moe_route", "bias", bias, e, torch.float32)
+    idx = torch.empty(*logits.shape[:-1], max(k, 0), dtype=torch.int32, device=dev)
+    w = torch.empty(*logits.shape[:-1], max(k, 0), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().kq_moe_route(_p(lg), _DT[lg.dtype], t, e, lg.stride(0), k, _SCORES[scoring], _p(bias),
+                                            n_groups, topk_groups, int(bool(norm_topk_prob)), scale, _p(idx), _p(w),
+                                            _stream(dev)), "moe_route")
+    return idx, w

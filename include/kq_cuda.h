@@ -326,6 +326,75 @@ int kq_quantized_matmul_chain(const kq_chain_problem *problems, int count, int x
  * synchronises `stream`.  Returns the word (0 = no device-side error). */
 int kq_workspace_error(void *workspace, int clear, void *stream);
 
+/* ---- serving step around the projections ------------------------------------
+ * A paged cache holds keys and values of all requests in pages of `page_size`
+ * tokens; a request's block table lists its pages.  Slot s is row
+ * s % page_size of page s / page_size.  The four calls below share the
+ * conventions above; a length, slot, position or page id on the device that
+ * contradicts the buffers is never followed: it is skipped and recorded in the
+ * workspace's error word (20 lengths, 21 no page left, 22 index out of range). */
+typedef struct kq_paged_cache {
+    void *k, *v; /* values of (page, row, head) at page * page_stride + row * row_stride + head * head_stride */
+    int dtype;   /* KQ_F16 or KQ_BF16 */
+    int64_t pages, page_size, kv_heads, dim;
+    int64_t page_stride, row_stride, head_stride; /* elements, multiples of 8; the same for k and v */
+} kq_paged_cache;
+
+/* Block tables, token slots and positions of a step, from the requests' lengths:
+ * request b has context_lens[b] tokens cached and query_lens[b] new ones; the
+ * pages it lacks are free_pages[first_b ...], in request order, written into its
+ * row of block_tables ([batch][table_width], row stride table_stride).
+ * cu_seqlens [batch + 1], seq_lens [batch] (context + new), slots / positions
+ * [n_tokens] (tokens past the last request: slot -1, position 0), pages_used [1].
+ * batch <= 8192.  Workspace: 256 bytes (the error word). */
+int kq_paged_plan(const int32_t *context_lens, const int32_t *query_lens, int64_t batch, int32_t *block_tables,
+                  int64_t table_stride, int64_t table_width, const int32_t *free_pages, int64_t n_free,
+                  int64_t page_size, int64_t n_tokens, int32_t *cu_seqlens, int32_t *seq_lens, int64_t *slots,
+                  int32_t *positions, int32_t *pages_used, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Rotary embedding of the new queries and keys, and the store of keys and values
+ * into their cache slots (slot < 0: none).  q [tokens][heads][dim], k and v
+ * [tokens][kv_heads][dim] with token and head strides (elements, multiples of 8);
+ * cos, sin [n_positions][rot / 2] f32; the first `rot` values of a head turn, in
+ * pairs (2i, 2i + 1) when interleaved, else (i, i + rot / 2).  dim and rot are
+ * multiples of 16.  q_out [tokens][heads][dim].  Workspace: 256 bytes. */
+int kq_rope_kv_write(const kq_paged_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                     const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                     int64_t v_token_stride, int64_t v_head_stride, int64_t tokens, int64_t heads, const float *cos,
+                     const float *sin, int64_t n_positions, int rot, int interleaved, const int32_t *positions,
+                     const int64_t *slots, void *q_out, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Attention of the new tokens of every request over its pages: request b's
+ * queries are rows cu_seqlens[b] .. cu_seqlens[b + 1] of q, its keys the first
+ * seq_lens[b] rows of its block table.  Row i of n sees the keys below
+ * limit = seq_len - n + i + 1 (all of them when not causal), and only the last
+ * `window` of those when window > 0 (causal only).  Scores are scale * q . k, then
+ * softcap * tanh(score / softcap) when softcap > 0.  out [tokens][heads][dim];
+ * lse [tokens][heads] f32 (natural log of the row's sum) or NULL.  Rows without
+ * keys, and tokens past cu_seqlens[batch], give 0 and -inf.  dim is 64, 128 or
+ * 256; heads a multiple of kv_heads.  max_query_len only picks the kernels: a
+ * longer request is still computed in full. */
+int kq_paged_attention(const kq_paged_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                       int64_t tokens, int64_t heads, const int32_t *block_tables, int64_t table_stride,
+                       int64_t table_width, const int32_t *seq_lens, const int32_t *cu_seqlens, int64_t batch,
+                       int64_t max_query_len, float scale, int causal, int64_t window, float softcap, void *out,
+                       float *lse, void *workspace, size_t workspace_bytes, void *stream);
+size_t kq_paged_attention_workspace_size(int64_t dim);
+
+/* Experts and weights of each token from router logits [t][e] (f32, f16 or bf16,
+ * row stride in elements): scores p = softmax (scoring 0) or sigmoid (1); the
+ * choice goes by p + bias (bias [e] f32 or NULL); with n_groups > 1 the groups of
+ * e / n_groups consecutive experts are ranked by the sum of their two best and
+ * only the first topk_groups are open.  idx, weights [t][k]: descending, ties to
+ * the lower index; weights are p of the chosen, divided by their sum when
+ * norm_topk_prob, times scale.  A NaN logit counts as -inf; a row whose chosen
+ * scores sum to 0 gets weights 0.  e <= 1024, k <= 32, n_groups <= 32. */
+#define KQ_SCORE_SOFTMAX 0
+#define KQ_SCORE_SIGMOID 1
+int kq_moe_route(const void *logits, int dtype, int64_t t, int64_t e, int64_t row_stride, int k, int scoring,
+                 const float *bias, int n_groups, int topk_groups, int norm_topk_prob, float scale, int32_t *idx,
+                 float *weights, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
