@@ -22,7 +22,7 @@ STAMP = os.path.join(HERE, "_build", "linked_config")
 LIB = os.path.join(HERE, "libkq_cuda.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 SOURCES = ["kq_dequant.cu", "kq_gemv.cu", "kq_moe.cu", "kq_capi.cu", "kq_noalloc.cu", "kq_gemm_sm100.cu", "kq_chain.cu", "kq_allreduce.cu",
-           "kq_serve.cu", "kq_attn.cu", "kq_serve_capi.cu"]
+           "kq_serve.cu", "kq_attn.cu", "kq_attn_sm100.cu", "kq_serve_capi.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
          "-Xptxas", "-warn-spills"]

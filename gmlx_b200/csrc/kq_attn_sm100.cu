@@ -1,0 +1,703 @@
+// kq_attn_sm100.cu -- attention of a chunk of new tokens over a paged cache on
+// the 5th-generation tensor cores (tcgen05, accumulators in TMEM).
+//
+// A tile is 128 packed rows of one request and kv head (tokens x the query heads
+// that share the kv head); scores S = Q K^T of 128 keys at a time go to TMEM,
+// a warpgroup turns them into probabilities P one row a thread (no shuffles),
+// P goes back to TMEM over S and feeds O += P V, which stays in TMEM.
+//
+//   head dim 64, 128: two tiles a block, each with its own warpgroup, S and O:
+//     the tensor core works on one tile while the other's softmax runs;
+//   head dim 256: O takes half of TMEM, so one tile a block with two S buffers:
+//     the tensor core computes the next S and the last P V meanwhile.
+//
+// Blocks are persistent, one an SM.  The units of work (128 keys of one pair of
+// tiles) stand in one line over all requests and every block takes an equal run
+// of them; what a run cuts off goes through f32 partial rows in the workspace,
+// joined by the last block to arrive, in block order.
+//
+// Warps 0-3 and 4-7: softmax of tile 0 and 1, and their results; warp 8: TMA of
+// queries and pages (a page's rows of one head and 64 values a box; boxes that
+// no row sees are read out of bounds, which fills zeros); warp 9: MMA issue.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <string.h>
+
+#include "kq_attn.cuh"
+
+namespace kq {
+namespace {
+
+constexpr int TM = 128, KT = 128;  // rows a tile, keys a unit
+constexpr int THREADS = 384;
+constexpr int SOFT_REGS = 216, OTHER_REGS = 72;  // 256 x 216 + 128 x 72 = 384 x 168, what the launch holds
+static_assert(256 * SOFT_REGS + 128 * OTHER_REGS <= THREADS * 168, "register split");
+
+template <int D> struct TL {
+    static constexpr int NT = D <= 128 ? 2 : 1;
+    static constexpr int Q_BYTES = TM * D * 2, KV_BYTES = KT * D * 2;
+    static constexpr int NB = (232448 - 2048 - NT * Q_BYTES) / KV_BYTES > 6 ? 6 : (232448 - 2048 - NT * Q_BYTES) / KV_BYTES;
+    static constexpr int OFF_KV = NT * Q_BYTES, OFF_BAR = OFF_KV + NB * KV_BYTES;
+    static constexpr int SMEM = OFF_BAR + 256 + 1024;
+    static constexpr int S_COL = 0, O_COL = 2 * KT;  // S buffers, then O
+    static constexpr int PART = TM * (D + 2);        // floats of a tile's partial rows
+};
+
+struct TileArgs {
+    AttnArgs a;
+    int box_rows;    // rows of a page box
+    int tile_tok;    // tokens a tile: 128 / G
+    uint32_t q_tx;   // bytes of a tile's queries
+};
+
+__device__ __forceinline__ uint64_t gtimer() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Bounded wait (2 s): on expiry the error is recorded, the block's abort flag
+// stops all further issue, and every loop runs out.
+__device__ __forceinline__ bool wait_b(uint64_t *bar, uint32_t par, volatile int *abort, int *err, int code) {
+    uint64_t t0 = 0;
+    for (uint32_t i = 1;; i++) {
+        if (mbar_try_wait(bar, par)) return true;
+        if ((i & 1023) == 0) {
+            if (*abort) return false;
+            const uint64_t now = gtimer();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > 2000000000ull) {
+                *abort = 1;
+                atomicCAS(err, 0, code);
+                return false;
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void tma_4d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, int c0, int c1, int c2, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Shared-memory descriptors, SWIZZLE_128B, 8-row groups 1024 B apart.  The value
+// tile is read along its rows' values (MN-major): its 64-value column blocks are
+// KT * 128 B apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(KT * 128 / 16) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+template <bool F16> __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
+    const uint32_t fmt = F16 ? 0u : 1u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc)
+                 : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+#define KQ_R32(r, o) \
+    "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), \
+        "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), \
+        "=r"(r[o + 15]), "=r"(r[o + 16]), "=r"(r[o + 17]), "=r"(r[o + 18]), "=r"(r[o + 19]), "=r"(r[o + 20]), "=r"(r[o + 21]), \
+        "=r"(r[o + 22]), "=r"(r[o + 23]), "=r"(r[o + 24]), "=r"(r[o + 25]), "=r"(r[o + 26]), "=r"(r[o + 27]), "=r"(r[o + 28]), \
+        "=r"(r[o + 29]), "=r"(r[o + 30]), "=r"(r[o + 31])
+#define KQ_U32(r, o) \
+    "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]), \
+        "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]), "r"(r[o + 14]), \
+        "r"(r[o + 15]), "r"(r[o + 16]), "r"(r[o + 17]), "r"(r[o + 18]), "r"(r[o + 19]), "r"(r[o + 20]), "r"(r[o + 21]), \
+        "r"(r[o + 22]), "r"(r[o + 23]), "r"(r[o + 24]), "r"(r[o + 25]), "r"(r[o + 26]), "r"(r[o + 27]), "r"(r[o + 28]), \
+        "r"(r[o + 29]), "r"(r[o + 30]), "r"(r[o + 31])
+#define KQ_LIST32 \
+    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
+
+// 32 columns of this warp's 32 lanes; the registers hold them after tmem_wait_ld
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " KQ_LIST32 ", [%32];" : KQ_R32(r, 0) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " KQ_LIST32 ";" ::KQ_U32(r, 0), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// orders every use of r behind the wait before it
+__device__ __forceinline__ void pin(uint32_t &r) { asm volatile("" : "+r"(r)); }
+
+// One block's share of a pair of tiles, the same in every warp's walk.
+struct Seg {
+    int q0, n, len;        // the request
+    int b, h, tok0;        // first token of the pair
+    int lo, hi;            // keys its rows see
+    int lo_tile, tiles;    // key tiles of the pair
+    int k0, k1;            // this block's share of them
+    int c[2];              // key tiles of each tile of rows in the share
+    int64_t u0;            // first unit of the pair
+    int units;
+};
+
+template <int D> struct Walk {
+    static constexpr int NT = TL<D>::NT;
+    const TileArgs &p;
+    int64_t u, ue, before;
+    Request rq;
+    int b, qt;  // request, pair
+    bool bad;
+
+    __device__ __forceinline__ static int pair_units(const TileArgs &p, const Request &r, int qt, int &lo, int &hi) {
+        const int t0 = qt * NT * p.tile_tok, t1 = min(r.n, t0 + NT * p.tile_tok);
+        key_range(p.a, r, t0, t1, lo, hi);
+        return max(1, (hi + KT - 1) / KT - lo / KT);
+    }
+    __device__ __forceinline__ static int pairs(const TileArgs &p, const Request &r) {
+        const int64_t rows = (int64_t)r.n * p.a.G;
+        if (rows == 0 || rows > p.a.max_rows || rows < p.a.min_rows) return 0;
+        return (r.n + NT * p.tile_tok - 1) / (NT * p.tile_tok);
+    }
+    __device__ __forceinline__ static int64_t request_units(const TileArgs &p, const Request &r) {
+        const int n = pairs(p, r);
+        int64_t s = 0;
+        int lo, hi;
+        for (int i = 0; i < n; i++) s += pair_units(p, r, i, lo, hi);
+        return s * p.a.Hk;
+    }
+
+    __device__ __forceinline__ Walk(const TileArgs &p, int64_t ub, int64_t ue, int b0, int64_t before0)
+        : p(p), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
+        if (u < ue) rq = load_request(p.a, b, bad);
+    }
+    __device__ __forceinline__ bool next(Seg &s) {
+        if (u >= ue) return false;
+        int lo, hi, t;
+        for (;;) {  // the pair that holds unit u
+            if (qt < pairs(p, rq)) {
+                t = pair_units(p, rq, qt, lo, hi);
+                if (u < before + (int64_t)t * p.a.Hk) break;
+                before += (int64_t)t * p.a.Hk;
+                qt++;
+            } else {
+                qt = 0;
+                rq = load_request(p.a, ++b, bad);
+            }
+        }
+        s.q0 = rq.q0, s.n = rq.n, s.len = rq.len, s.b = b, s.lo = lo, s.hi = hi;
+        s.h = (int)((u - before) / t);
+        s.u0 = before + (int64_t)s.h * t;
+        s.units = t;
+        s.tok0 = qt * NT * p.tile_tok;
+        s.lo_tile = lo / KT;
+        s.tiles = (hi + KT - 1) / KT - s.lo_tile;
+        if (hi <= lo) s.tiles = 0;
+        s.k0 = (int)(u - s.u0), s.k1 = (int)min((int64_t)t, ue - s.u0);
+        u = s.u0 + s.k1;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int t0 = s.tok0 + i * p.tile_tok, t1 = min(rq.n, t0 + p.tile_tok);
+            int l, e;
+            key_range(p.a, rq, t0, t1, l, e);
+            const int own = i < NT && t0 < rq.n && e > l ? (e + KT - 1) / KT - s.lo_tile : 0;
+            s.c[i] = max(0, min(min(s.k1, s.tiles), own) - s.k0);
+        }
+        return true;
+    }
+};
+
+template <bool F16, int D, bool CAP>
+__global__ void __launch_bounds__(THREADS, 1)
+    tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TileArgs p) {
+    using L = TL<D>;
+    constexpr int NT = L::NT, NB = L::NB;
+    const AttnArgs &a = p.a;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *kv_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *kv_empty = kv_full + NB;
+    uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_full = p_full + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int *s_last = reinterpret_cast<volatile int *>(tmem_slot + 2);  // one a tile
+    int64_t *s_sum = reinterpret_cast<int64_t *>(smem);  // before the first copy arrives there
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < NB; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
+        mbar_init(q_full, 1), mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_full[i], 1);
+        *s_abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // units of each thread's run of requests (b == B: the padding tokens)
+    bool bad = false;
+    const int nb = a.B + 1, per = (nb + THREADS - 1) / THREADS;
+    int64_t mine = 0;
+    for (int i = 0; i < per; i++) {
+        const int b = tid * per + i;
+        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad));
+    }
+    s_sum[tid] = mine;
+    if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = *tmem_slot;
+    if (warp == 0) {
+        int64_t base = 0;
+        for (int w = 0; w < THREADS / 32; w++) {
+            int64_t v = s_sum[w * 32 + lane];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += x;
+            }
+            s_sum[w * 32 + lane] = v + base;
+            base += __shfl_sync(0xffffffffu, v, 31);
+        }
+    }
+    __syncthreads();
+    const int64_t total = s_sum[THREADS - 1];
+    const int grid = (int)min((int64_t)gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
+    const bool work = (int)blockIdx.x < grid;
+    const int64_t ub = work ? unit_begin(total, blockIdx.x, grid) : 0, ue = work ? unit_begin(total, blockIdx.x + 1, grid) : 0;
+    int run = 0, run_hi = THREADS - 1;
+    while (run < run_hi) {
+        const int mid = (run + run_hi) >> 1;
+        if (s_sum[mid] > ub) run_hi = mid;
+        else run = mid + 1;
+    }
+    Walk<D> walk(p, ub, ue, run * per, run ? s_sum[run - 1] : 0);
+    Seg s;
+    fence_async_shared();
+    __syncthreads();
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
+        if (warp == 8) {  // ---- TMA
+            const int rows = p.box_rows, nrow = KT / rows, nbox = nrow * (D / 64);
+            bool bad_page = false;
+            uint32_t fills = 0, items = 0;
+            while (walk.next(s)) {
+                const int n = max(s.c[0], s.c[1]);
+                if (n == 0) continue;
+                wait_b(q_empty, (items & 1) ^ 1, s_abort, a.err, 31);
+                items++;
+                if (lane == 0) {
+                    const int live = s.c[NT - 1] > 0 ? NT : 1;
+                    mbar_arrive_expect_tx(q_full, live * p.q_tx);
+                    if (!*s_abort)
+                        for (int t = 0; t < live; t++)
+                            for (int d = 0; d < D / 64; d++)
+                                tma_3d(smem + t * L::Q_BYTES + d * TM * 128, &tm_q, d * 64, s.h * a.G, s.q0 + s.tok0 + t * p.tile_tok, q_full);
+                }
+                const int32_t *bt = a.table + (int64_t)s.b * a.table_stride;
+                for (int j = 0; j < n; j++) {
+                    const int tile0 = (s.lo_tile + s.k0 + j) * KT;
+                    for (int kv = 0; kv < 2; kv++, fills++) {
+                        const int slot = fills % NB;
+                        wait_b(&kv_empty[slot], ((fills / NB) & 1) ^ 1, s_abort, a.err, 32);
+                        if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], L::KV_BYTES);
+                        __syncwarp();
+                        if (*s_abort) continue;
+                        for (int i = lane; i < nbox; i += 32) {
+                            const int r = i % nrow, d = i / nrow, key = tile0 + r * rows;
+                            int page = a.n_pages, col = 0;  // out of bounds: zeros
+                            if (key < s.hi && key + rows > s.lo) {
+                                col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
+                                const int id = bt[col];
+                                if ((unsigned)id < (unsigned)a.n_pages) page = id;
+                                else bad_page = true;
+                            }
+                            tma_4d(smem + L::OFF_KV + slot * L::KV_BYTES + d * KT * 128 + r * rows * 128, kv ? &tm_v : &tm_k, d * 64,
+                                   key - col * a.page < a.page ? max(0, key - col * a.page) : 0, s.h, page, &kv_full[slot]);
+                        }
+                    }
+                }
+            }
+            if (bad_page) atomicCAS(a.err, 0, ERR_INDEX);
+            if (*s_abort)  // nothing consumes what is still in flight: let it land before the block ends
+                for (uint32_t f = fills > NB ? fills - NB : 0; f < fills; f++)
+                    mbar_wait(&kv_full[f % NB], (f / NB) & 1, 1u << 20);
+        } else if (warp == 9) {  // ---- MMA
+            constexpr uint32_t id_s = idesc<F16>(KT, false), id_o = idesc<F16>(D, true);
+            uint32_t takes = 0, items = 0, np[2] = {0, 0}, ns = 0;
+            while (walk.next(s)) {
+                const int n = max(s.c[0], s.c[1]);
+                if (n == 0) continue;
+                wait_b(q_full, items & 1, s_abort, a.err, 33);
+                items++;
+                auto qk = [&](int t, int buf, uint32_t take) {  // S[buf] = Q[t] K^T
+                    if (lane == 0 && !*s_abort) {
+                        const uint32_t sq = smem_u32(smem + t * L::Q_BYTES), sk = smem_u32(smem + L::OFF_KV + (take % NB) * L::KV_BYTES);
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; kk++)
+                            mma_ss(tmem + L::S_COL + buf * KT, desc_k(sq + (kk >> 2) * TM * 128 + (kk & 3) * 32),
+                                   desc_k(sk + (kk >> 2) * KT * 128 + (kk & 3) * 32), id_s, kk ? 1u : 0u);
+                    }
+                    if (lane == 0) commit(&s_full[buf]);
+                };
+                auto pv = [&](int t, int buf, uint32_t take, bool acc) {  // O[t] += P[buf] V
+                    if (lane == 0 && !*s_abort) {
+                        const uint32_t sv = smem_u32(smem + L::OFF_KV + (take % NB) * L::KV_BYTES);
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; kk++)
+                            mma_ts(tmem + L::O_COL + t * D, tmem + L::S_COL + buf * KT + kk * 8, desc_mn(sv + kk * 2048), id_o,
+                                   acc || kk ? 1u : 0u);
+                    }
+                    if (lane == 0) commit(&o_full[t]);
+                };
+                auto full = [&](uint32_t take) {
+                    wait_b(&kv_full[take % NB], (take / NB) & 1, s_abort, a.err, 34);
+                    tc_after();
+                };
+                auto release = [&](uint32_t take) {
+                    if (lane == 0) commit(&kv_empty[take % NB]);
+                };
+                auto values = [&](uint32_t take, int j) {  // a page's rows that no row sees may hold anything: 0 * NaN
+                    full(take);
+                    const int tile0 = (s.lo_tile + s.k0 + j) * KT;
+                    if (tile0 < s.lo || tile0 + KT > s.hi) {
+                        uint8_t *sv = smem + L::OFF_KV + (take % NB) * L::KV_BYTES;
+                        const int from = min(max(s.hi - tile0, 0), KT), to = min(max(s.lo - tile0, 0), KT);
+                        for (int i = lane; i < KT * 8; i += 32) {
+                            const int r = i >> 3;
+                            if (r >= to && r < from) continue;
+#pragma unroll
+                            for (int d = 0; d < D / 64; d++)
+                                *reinterpret_cast<uint4 *>(sv + d * KT * 128 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async_shared();
+                        __syncwarp();
+                    }
+                };
+                if constexpr (NT == 2) {
+                    full(takes);
+#pragma unroll
+                    for (int t = 0; t < 2; t++)
+                        if (s.c[t] > 0) qk(t, t, takes);
+                    release(takes);
+                    if (n == 1 && lane == 0) commit(q_empty);
+                    for (int j = 0; j < n; j++) {
+                        const uint32_t tv = takes + 2 * j + 1, tk = tv + 1;
+                        values(tv, j);
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            if (j < s.c[t]) {
+                                wait_b(&p_full[t], np[t]++ & 1, s_abort, a.err, 35);
+                                tc_after();
+                                pv(t, t, tv, j > 0);
+                            }
+                            if (t == 0 && j + 1 < n) full(tk);
+                            if (j + 1 < s.c[t]) qk(t, t, tk);
+                        }
+                        release(tv);
+                        if (j + 1 < n) release(tk);
+                        if (j + 2 == n && lane == 0) commit(q_empty);
+                    }
+                } else {
+                    full(takes);
+                    qk(0, ns & 1, takes);
+                    release(takes);
+                    if (n == 1 && lane == 0) commit(q_empty);
+                    for (int j = 0; j < n; j++, ns++) {
+                        const uint32_t tv = takes + 2 * j + 1, tk = tv + 1;
+                        values(tv, j);
+                        if (j + 1 < n) {
+                            full(tk);
+                            qk(0, (ns + 1) & 1, tk);
+                            release(tk);
+                            if (j + 2 == n && lane == 0) commit(q_empty);
+                        }
+                        wait_b(&p_full[ns & 1], np[ns & 1]++ & 1, s_abort, a.err, 35);
+                        tc_after();
+                        pv(0, ns & 1, tv, j > 0);
+                        release(tv);
+                    }
+                }
+                takes += 2 * n;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
+        // ---- softmax: this thread's row of tile t
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 * (warp % 4)
+        const uint32_t o_addr = tmem + lanes + L::O_COL + (NT == 2 ? t : 0) * D;
+        const float sl2 = CAP ? 1.0f : a.scale * LOG2E;
+        const float cap_in = CAP ? 2.0f * LOG2E * a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
+        const float slack = 8.0f / sl2;  // the reference lags the maximum by up to 2^8
+        uint32_t nsf = 0, no = 0;        // S tiles and P V products of this tile so far
+        while (t < NT && walk.next(s)) {
+            const int tok = s.tok0 + t * p.tile_tok + row / a.G;
+            const int live_tok = min(s.n, s.tok0 + (t + 1) * p.tile_tok);
+            const bool live = row < p.tile_tok * a.G && tok < live_tok;
+            const int shift = s.len - s.n + 1, mtok = min(tok, live_tok - 1);
+            const int lim = a.causal ? shift + mtok : s.len, low = a.window ? lim - a.window : 0;
+            // keys that every row of the tile sees
+            const int all_hi = a.causal ? shift + s.tok0 + t * p.tile_tok : s.len, all_lo = a.window ? shift + live_tok - 1 - a.window : 0;
+            float ref = -INFINITY, l = 0.f;
+            const int c = s.c[t];
+            for (int j = 0; j < c; j++) {
+                const int buf = NT == 2 ? t : (int)(nsf & 1), key0 = (s.lo_tile + s.k0 + j) * KT;
+                const uint32_t s_addr = tmem + lanes + L::S_COL + buf * KT;
+                wait_b(&s_full[buf], NT == 2 ? nsf & 1 : (nsf >> 1) & 1, s_abort, a.err, 36);
+                nsf++;
+                tc_after();
+                uint32_t x[KT];
+#pragma unroll
+                for (int i = 0; i < KT; i += 32) tmem_ld32(s_addr + i, x + i);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < KT; i++) pin(x[i]);
+                float *f = reinterpret_cast<float *>(x);
+                if (CAP) {
+#pragma unroll
+                    for (int i = 0; i < KT; i++) f[i] = soft_cap(f[i], cap_in, cap_out);
+                }
+                if (key0 + KT > all_hi || key0 < all_lo) {
+                    const int hi_i = lim - key0, lo_i = low - key0;
+#pragma unroll
+                    for (int i = 0; i < KT; i++) f[i] = i < hi_i && i >= lo_i ? f[i] : -INFINITY;
+                }
+                float m0 = f[0], m1 = f[1], m2 = f[2], m3 = f[3];
+#pragma unroll
+                for (int i = 4; i < KT; i += 4) {
+                    m0 = fmaxf(m0, f[i]), m1 = fmaxf(m1, f[i + 1]);
+                    m2 = fmaxf(m2, f[i + 2]), m3 = fmaxf(m3, f[i + 3]);
+                }
+                const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+                // O and l are kept relative to `ref`, which follows the maximum only when
+                // that has outgrown it by 2^8: f32 holds the excess exactly, P's type too
+                const bool grow = j == 0 ? true : mx > ref + slack;
+                if (__any_sync(0xffffffffu, grow && j > 0)) {
+                    const float to = grow ? mx : ref;
+                    const float k = ref == -INFINITY ? (grow ? 0.f : 1.f) : ex2((ref - to) * sl2);
+                    l *= k;
+                    ref = to;
+                    wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 37);
+                    tc_after();
+#pragma unroll
+                    for (int d = 0; d < D; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld32(o_addr + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) {
+                            pin(o[i]);
+                            o[i] = __float_as_uint(__uint_as_float(o[i]) * k);
+                        }
+                        tmem_st32(o_addr + d, o);
+                    }
+                } else if (j == 0) ref = mx;
+                const float base = ref == -INFINITY ? 0.f : ref * sl2;
+                float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+                for (int g = 0; g < KT; g += 64) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const float p0 = ex2(fmaf(f[g + 2 * i], sl2, -base)), p1 = ex2(fmaf(f[g + 2 * i + 1], sl2, -base));
+                        l0 += p0, l1 += p1;
+                        // rounded to the values' type for the product; the sum stays in f32
+                        pk[i] = pack_half<F16>(p0, p1);
+                    }
+                    tmem_st32(s_addr + g / 2, pk);
+                }
+                l += l0 + l1;
+                tmem_wait_st();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[buf]);
+                no++;
+            }
+            // ---- the tile's rows, or this block's part of them
+            const int first = unit_block(total, s.u0, grid), last = unit_block(total, s.u0 + s.units - 1, grid);
+            const bool has_tile = s.tok0 + t * p.tile_tok < s.n;
+            if (!has_tile) continue;
+            if (c > 0) {
+                wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 38);
+                tc_after();
+            }
+            const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row % a.G;
+            uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + orow * D;
+            const float ml = ref * sl2;  // log2 units
+            if (first == last) {
+                const float inv = l > 0.f ? 1.0f / l : 0.f;
+#pragma unroll
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t o[32];
+                    if (c > 0) {
+                        tmem_ld32(o_addr + d, o);
+                        tmem_wait_ld();
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        pin(o[i]);
+                        if (c == 0) o[i] = 0u;
+                    }
+                    if (live)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 w;
+                            w.x = pack_half<F16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                            w.y = pack_half<F16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                            w.z = pack_half<F16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                            w.w = pack_half<F16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                            *reinterpret_cast<uint4 *>(dst + d + i) = w;
+                        }
+                }
+                if (live && a.lse) a.lse[orow] = l > 0.f ? ml * LN2 + logf(l) : -INFINITY;
+                continue;
+            }
+            // partial rows: m, l [128], then float4 [D / 4][128] (a warp's rows side by side)
+            float *part = a.part + (int64_t)((blockIdx.x * 2 + (s.k0 == 0 ? 1 : 0)) * NT + t) * L::PART;
+            part[row] = l > 0.f ? ml : -INFINITY;
+            part[TM + row] = l;
+            if (c > 0) {
+#pragma unroll
+                for (int d = 0; d < D; d += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + d, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) pin(o[i]);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4 *>(part + 2 * TM + ((d + i) / 4 * TM + row) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                }
+            }
+            __threadfence();
+            named_bar_sync(1 + t, 128);
+            if (row == 0) {
+                const int n = atomicAdd(a.cnt + first * 2 + t, 1);
+                s_last[t] = n == last - first;
+                if (n == last - first) a.cnt[first * 2 + t] = 0;
+            }
+            named_bar_sync(1 + t, 128);
+            const bool join = s_last[t];
+            named_bar_sync(1 + t, 128);  // s_last is read before the next tile's
+            if (!join) continue;
+            __threadfence();
+            float mm = -INFINITY;
+            for (int b = first; b <= last; b++)
+                mm = fmaxf(mm, __ldcg(a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART + row));
+            float ll = 0.f;
+            for (int b = first; b <= last; b++) {
+                const float *q = a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART;
+                const float mb = __ldcg(q + row);
+                ll += mb == -INFINITY ? 0.f : ex2(mb - mm) * __ldcg(q + TM + row);
+            }
+            const float inv = ll > 0.f ? 1.0f / ll : 0.f;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 64) {
+                float4 acc[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int b = first; b <= last; b++) {
+                    const float *q = a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART;
+                    const float mb = __ldcg(q + row);
+                    if (mb == -INFINITY) continue;
+                    const float w = ex2(mb - mm);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(q + 2 * TM) + (d / 4 + i) * TM + row);
+                        acc[i].x += w * v.x, acc[i].y += w * v.y, acc[i].z += w * v.z, acc[i].w += w * v.w;
+                    }
+                }
+                if (live)
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2)
+                        *reinterpret_cast<uint4 *>(dst + d + i * 4) =
+                            make_uint4(pack_half<F16>(acc[i].x * inv, acc[i].y * inv), pack_half<F16>(acc[i].z * inv, acc[i].w * inv),
+                                       pack_half<F16>(acc[i + 1].x * inv, acc[i + 1].y * inv), pack_half<F16>(acc[i + 1].z * inv, acc[i + 1].w * inv));
+            }
+            if (live && a.lse) a.lse[orow] = ll > 0.f ? mm * LN2 + logf(ll) : -INFINITY;
+        }
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+bool encode(CUtensorMap *m, bool f16, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
+    cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    return cuTensorMapEncodeTiled(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(base),
+                                  dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaStream_t st, bool &taken) {
+    using L = TL<D>;
+    TileArgs p;
+    p.a = a;
+    int rows = 1;  // the largest power of two that divides both a page and a tile
+    while (rows < KT && a.page % (rows * 2) == 0) rows *= 2;
+    p.box_rows = rows;
+    p.tile_tok = TM / a.G;
+    p.q_tx = (uint32_t)(p.tile_tok * a.G * D * 2);
+    CUtensorMap mq, mk, mv;
+    // a dimension of one entry has no stride of its own
+    auto bytes = [](int64_t s) { return (cuuint64_t)(s > 0 ? s * 2 : 16); };
+    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.Hq, (cuuint64_t)a.T}, qs[2] = {bytes(a.q_hs), bytes(a.q_ts)};
+    const cuuint32_t qb[3] = {64, (cuuint32_t)a.G, (cuuint32_t)p.tile_tok};
+    const cuuint64_t cd[4] = {(cuuint64_t)D, (cuuint64_t)a.page, (cuuint64_t)a.Hk, (cuuint64_t)a.n_pages};
+    const cuuint64_t cs[3] = {bytes(a.row_stride), bytes(a.head_stride), bytes(a.page_stride)};
+    const cuuint32_t cb[4] = {64, (cuuint32_t)rows, 1, 1};
+    taken = encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
+    if (!taken) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<F16, D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+    if (e != cudaSuccess) return e;
+    tiles_kernel<F16, D, CAP><<<num_sms(), THREADS, L::SMEM, st>>>(mq, mk, mv, p);
+    return cudaGetLastError();
+}
+
+template <bool F16, int D> cudaError_t launch_cap(const AttnArgs &a, cudaStream_t st, bool &taken) {
+    return a.softcap > 0.f ? launch<F16, D, true>(a, st, taken) : launch<F16, D, false>(a, st, taken);
+}
+
+}  // namespace
+
+size_t attn_tiles_part_bytes(int D) {
+    return (size_t)num_sms() * 2 * (D <= 128 ? 2 : 1) * TM * (D + 2) * sizeof(float);
+}
+
+cudaError_t launch_attn_tiles(const AttnArgs &a, int dtype, cudaStream_t st, bool &taken) {
+    taken = false;
+    if (a.G > TM) return cudaSuccess;
+    const bool f16 = dtype == F16;
+    switch (a.D) {
+        case 64: return f16 ? launch_cap<true, 64>(a, st, taken) : launch_cap<false, 64>(a, st, taken);
+        case 128: return f16 ? launch_cap<true, 128>(a, st, taken) : launch_cap<false, 128>(a, st, taken);
+        case 256: return f16 ? launch_cap<true, 256>(a, st, taken) : launch_cap<false, 256>(a, st, taken);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace kq

@@ -83,8 +83,14 @@ struct AttnArgs {
     int max_rows;  // requests with more packed rows (tokens x G) are another launch's
     int min_rows;  // requests with fewer too
 };
-// Bytes of `part` the launches need for this head count and dimension.
+// Bytes of `part` the launches need for this head dimension.
 size_t attn_part_bytes(int D);
+size_t attn_tiles_part_bytes(int D);
+// Few rows (kq_attn.cu): requests of any size, fast up to ROWS_MAX packed rows.
+constexpr int ROWS_MAX = 16;
 cudaError_t launch_attn_rows(const AttnArgs &a, int dtype, cudaStream_t st);
+// Chunks (kq_attn_sm100.cu).  taken = false, nothing launched: a layout that
+// the tensor maps cannot describe, or more than 128 query heads a kv head.
+cudaError_t launch_attn_tiles(const AttnArgs &a, int dtype, cudaStream_t st, bool &taken);
 
 }  // namespace kq

@@ -104,7 +104,9 @@ int kq_rope_kv_write(const kq_paged_cache *cache, const void *q, int64_t q_token
 }
 
 size_t kq_paged_attention_workspace_size(int64_t dim) {
-    return PART_OFF + (dim > 0 && dim <= 256 ? attn_part_bytes((int)dim) : 0);
+    if (dim < 1 || dim > 256) return PART_OFF;
+    const size_t rows = attn_part_bytes((int)dim), tiles = attn_tiles_part_bytes((int)dim);
+    return PART_OFF + (rows > tiles ? rows : tiles);
 }
 
 int kq_paged_attention(const kq_paged_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
@@ -123,8 +125,8 @@ int kq_paged_attention(const kq_paged_cache *cache, const void *q, int64_t q_tok
         return fail(KQ_ERR_SHAPE, "%s: %lld tokens, %lld requests, tables of %lld entries at stride %lld", what,
                     (long long)tokens, (long long)batch, (long long)table_width, (long long)table_stride);
     if (window < 0 || (window && !causal)) return fail(KQ_ERR_SHAPE, "%s: a window of %lld keys (>= 0, and causal only)", what, (long long)window);
-    if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(scale == scale) || !(scale < INFINITY && scale > -INFINITY))
-        return fail(KQ_ERR_SHAPE, "%s: scale %g, softcap %g", what, (double)scale, (double)softcap);
+    if (!(softcap >= 0.f) || !(softcap < INFINITY) || !(scale > 0.f && scale < INFINITY))
+        return fail(KQ_ERR_SHAPE, "%s: scale %g (positive), softcap %g (>= 0)", what, (double)scale, (double)softcap);
     if (!aligned(q, q_token_stride, q_head_stride) || !aligned(out, 0, 0))
         return fail(KQ_ERR_ALIGN, "%s: bases must be 16-byte aligned and strides multiples of 8", what);
     if (int rc = need_workspace(workspace, workspace_bytes, kq_paged_attention_workspace_size(d), what)) return rc;
@@ -145,6 +147,19 @@ int kq_paged_attention(const kq_paged_cache *cache, const void *q, int64_t q_tok
     a.out = out, a.lse = lse;
     a.err = (int *)workspace, a.cnt = (int *)((char *)workspace + 256), a.part = (float *)((char *)workspace + PART_OFF);
     a.min_rows = 0, a.max_rows = 0x7fffffff;
+    if (tokens == 0) return KQ_OK;
+    // Up to ROWS_MAX packed rows a request is bound by reading its keys, and the
+    // register tiles do that; longer ones go to the tensor-core tiles.  A batch may
+    // hold both, so each launch then takes its kind of request, told apart by the
+    // lengths on the device; a single request needs the tiles alone.
+    if (max_query_len * a.G > ROWS_MAX) {
+        bool taken = false;
+        if (batch > 1) a.min_rows = ROWS_MAX + 1;
+        if (int rc = done(launch_attn_tiles(a, cache->dtype, (cudaStream_t)stream, taken), what)) return rc;
+        if (taken && batch <= 1) return KQ_OK;
+        if (taken) a.max_rows = ROWS_MAX;
+        a.min_rows = 0;
+    }
     return done(launch_attn_rows(a, cache->dtype, (cudaStream_t)stream), what);
 }
 

@@ -36,7 +36,6 @@ on the current torch CUDA stream.
 from __future__ import annotations
 
 import ctypes as _ct
-import math
 from typing import NamedTuple
 
 import torch
@@ -879,7 +878,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     ``heads / kv_heads`` query heads in a row.  Row ``i`` of ``n`` sees the keys
     below ``seq_len - n + i + 1`` (all of the request's when not ``causal``), and
     only the last ``window`` of those when ``window > 0``.  Scores are
-    ``scale * q.k`` (default ``dim ** -0.5``), capped as
+    ``scale * q.k`` (``scale > 0``, default ``dim ** -0.5``), capped as
     ``softcap * tanh(score / softcap)`` when ``softcap > 0``; scores, maxima and
     sums are held in f32.  Returns ``out`` like ``q``, with ``return_lse`` also
     the log of each row's sum, f32 ``[tokens, heads]``.
@@ -907,8 +906,6 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     b = seq.shape[0]
     cu = _vector(what, "cu_seqlens", cu_seqlens, b + 1, torch.int32)
     stride, width = _table(what, block_tables, b)
-    if not math.isfinite(scale) or not math.isfinite(softcap):
-        raise ValueError(f"{what}: scale {scale}, softcap {softcap}")
     out = torch.empty(t, hq, cache.dim, dtype=q.dtype, device=dev)
     lse = torch.empty(t, hq, dtype=torch.float32, device=dev) if return_lse else None
     with torch.cuda.device(dev):

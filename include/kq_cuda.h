@@ -368,7 +368,7 @@ int kq_rope_kv_write(const kq_paged_cache *cache, const void *q, int64_t q_token
  * queries are rows cu_seqlens[b] .. cu_seqlens[b + 1] of q, its keys the first
  * seq_lens[b] rows of its block table.  Row i of n sees the keys below
  * limit = seq_len - n + i + 1 (all of them when not causal), and only the last
- * `window` of those when window > 0 (causal only).  Scores are scale * q . k, then
+ * `window` of those when window > 0 (causal only).  Scores are scale * q . k (scale > 0), then
  * softcap * tanh(score / softcap) when softcap > 0.  out [tokens][heads][dim];
  * lse [tokens][heads] f32 (natural log of the row's sum) or NULL.  Rows without
  * keys, and tokens past cu_seqlens[batch], give 0 and -inf.  dim is 64, 128 or
