@@ -3,11 +3,12 @@
 //
 // A tile is 128 packed rows of one request and kv head (tokens x the query heads
 // that share the kv head); scores S = Q K^T of 128 keys at a time go to TMEM,
-// a warpgroup turns them into probabilities P one row a thread (no shuffles),
-// P goes back to TMEM over S and feeds O += P V, which stays in TMEM.
+// eight warps turn them into probabilities P, two threads a row with 64 keys
+// each (no shuffles), P goes back to TMEM over S and feeds O += P V, which stays
+// in TMEM.
 //
-//   head dim 64, 128: two tiles a block, each with its own warpgroup, S and O:
-//     the tensor core works on one tile while the other's softmax runs;
+//   head dim 64, 128: two tiles a block, each with its own warps, S and O: the
+//     tensor core works on one tile while the other's softmax runs;
 //   head dim 256: O takes half of TMEM, so one tile a block with two S buffers:
 //     the tensor core computes the next S and the last P V meanwhile.
 //
@@ -16,9 +17,11 @@
 // of them; what a run cuts off goes through f32 partial rows in the workspace,
 // joined by the last block to arrive, in block order.
 //
-// Warps 0-3 and 4-7: softmax of tile 0 and 1, and their results; warp 8: TMA of
+// Warps 0-7 and 8-15: softmax of tile 0 and 1, and their results; warp 16: TMA of
 // queries and pages (a page's rows of one head and 64 values a box; boxes that
-// no row sees are read out of bounds, which fills zeros); warp 9: MMA issue.
+// no row sees are read out of bounds, which fills zeros); warp 17: MMA issue;
+// warp 18: walks the block's run of units and hands its shares of tile pairs to
+// the others through two slots in shared memory (their registers hold scores).
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -30,16 +33,17 @@ namespace kq {
 namespace {
 
 constexpr int TM = 128, KT = 128;  // rows a tile, keys a unit
-constexpr int THREADS = 384;
-constexpr int SOFT_REGS = 216, OTHER_REGS = 72;  // 256 x 216 + 128 x 72 = 384 x 168, what the launch holds
-static_assert(256 * SOFT_REGS + 128 * OTHER_REGS <= THREADS * 168, "register split");
+constexpr int SOFT_WARPS = 16, TMA_WARP = 16, MMA_WARP = 17, WALK_WARP = 18, THREADS = 640;
+constexpr int HC = KT / 2;  // keys of a row that one thread handles
 
 template <int D> struct TL {
     static constexpr int NT = D <= 128 ? 2 : 1;
     static constexpr int Q_BYTES = TM * D * 2, KV_BYTES = KT * D * 2;
-    static constexpr int NB = (232448 - 2048 - NT * Q_BYTES) / KV_BYTES > 6 ? 6 : (232448 - 2048 - NT * Q_BYTES) / KV_BYTES;
+    static constexpr int NB = (232448 - 3584 - NT * Q_BYTES) / KV_BYTES > 6 ? 6 : (232448 - 3584 - NT * Q_BYTES) / KV_BYTES;
     static constexpr int OFF_KV = NT * Q_BYTES, OFF_BAR = OFF_KV + NB * KV_BYTES;
-    static constexpr int SMEM = OFF_BAR + 256 + 1024;
+    static constexpr int OFF_X = OFF_BAR + 256;  // maxima and sums that the two threads of a row exchange
+    static constexpr int OFF_SEG = OFF_X + 2 * 2 * TM * 4;
+    static constexpr int SMEM = OFF_SEG + 256 + 1024;
     static constexpr int S_COL = 0, O_COL = 2 * KT;  // S buffers, then O
     static constexpr int PART = TM * (D + 2);        // floats of a tile's partial rows
 };
@@ -127,28 +131,94 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
         "=r"(r[o + 15]), "=r"(r[o + 16]), "=r"(r[o + 17]), "=r"(r[o + 18]), "=r"(r[o + 19]), "=r"(r[o + 20]), "=r"(r[o + 21]), \
         "=r"(r[o + 22]), "=r"(r[o + 23]), "=r"(r[o + 24]), "=r"(r[o + 25]), "=r"(r[o + 26]), "=r"(r[o + 27]), "=r"(r[o + 28]), \
         "=r"(r[o + 29]), "=r"(r[o + 30]), "=r"(r[o + 31])
-#define KQ_U32(r, o) \
-    "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]), \
-        "r"(r[o + 8]), "r"(r[o + 9]), "r"(r[o + 10]), "r"(r[o + 11]), "r"(r[o + 12]), "r"(r[o + 13]), "r"(r[o + 14]), \
-        "r"(r[o + 15]), "r"(r[o + 16]), "r"(r[o + 17]), "r"(r[o + 18]), "r"(r[o + 19]), "r"(r[o + 20]), "r"(r[o + 21]), \
-        "r"(r[o + 22]), "r"(r[o + 23]), "r"(r[o + 24]), "r"(r[o + 25]), "r"(r[o + 26]), "r"(r[o + 27]), "r"(r[o + 28]), \
-        "r"(r[o + 29]), "r"(r[o + 30]), "r"(r[o + 31])
 #define KQ_LIST32 \
     "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
 
-// 32 columns of this warp's 32 lanes; the registers hold them after tmem_wait_ld
+#define KQ_R16(r) \
+    "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), \
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+#define KQ_U16(r) \
+    "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), \
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+#define KQ_LIST16 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}"
+
+// 32 (16) columns of this warp's 32 lanes; the registers hold them after tmem_wait_ld
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " KQ_LIST32 ", [%32];" : KQ_R32(r, 0) : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], " KQ_LIST32 ";" ::KQ_U32(r, 0), "r"(addr) : "memory");
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t *r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 " KQ_LIST16 ", [%16];" : KQ_R16(r) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], " KQ_LIST16 ";" ::KQ_U16(r), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // orders every use of r behind the wait before it
 __device__ __forceinline__ void pin(uint32_t &r) { asm volatile("" : "+r"(r)); }
 
-// One block's share of a pair of tiles, the same in every warp's walk.
+// Arithmetic on pairs of f32 in a 64-bit register.
+__device__ __forceinline__ uint64_t pack2u(uint32_t x, uint32_t y) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(x), "r"(y));
+    return v;
+}
+__device__ __forceinline__ uint64_t pack2f(float x, float y) { return pack2u(__float_as_uint(x), __float_as_uint(y)); }
+__device__ __forceinline__ void unpack2f(uint64_t v, float &x, float &y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+    uint64_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(x), "l"(y), "l"(z));
+    return v;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
+__device__ __forceinline__ float max3f(uint32_t x, uint32_t y, uint32_t z) {
+    float v;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(__uint_as_float(x)), "f"(__uint_as_float(y)), "f"(__uint_as_float(z)));
+    return v;
+}
+
+// 2^x of a pair.  The SFU gives 16 results a clock and SM, half of what the
+// tensor core's scores ask for, so POLY of 8 pairs take the FMA pipe instead:
+// x = n + f with |f| <= 1/2 (n by adding 1.5 * 2^23), 2^f by the polynomial of
+// degree 4 whose largest relative error on that interval is smallest (2.7e-6,
+// fitted by exchange of the extrema), and n added to the exponent.
+constexpr int POLY = 3;
+__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
+    float u, v;
+    unpack2f(x, u, v);
+    return pack2f(ex2(u), ex2(v));
+}
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+    float u, v;
+    unpack2f(x, u, v);
+    x = pack2f(fmaxf(u, -126.0f), fmaxf(v, -126.0f));
+    const uint64_t big = pack2f(12582912.0f, 12582912.0f), nbig = pack2f(-12582912.0f, -12582912.0f), none = pack2f(-1.0f, -1.0f);
+    const uint64_t n = add2(x, big), f = fma2(add2(n, nbig), none, x);
+    uint64_t y = fma2(f, pack2f(0.009570102207362652f, 0.009570102207362652f), pack2f(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(y, f, pack2f(0.240247443318367f, 0.240247443318367f));
+    y = fma2(y, f, pack2f(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(y, f, pack2f(0.9999992847442627f, 0.9999992847442627f));
+    float n0, n1, y0, y1;
+    unpack2f(n, n0, n1);
+    unpack2f(y, y0, y1);
+    return pack2u(__float_as_uint(y0) + (__float_as_uint(n0) << 23), __float_as_uint(y1) + (__float_as_uint(n1) << 23));
+}
+
+// Barrier of a warp pair (64 threads) that gives the OR of their predicates.
+__device__ __forceinline__ bool bar_or(int id, bool v) {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+                 : "=r"(r)
+                 : "r"(id), "r"((uint32_t)v)
+                 : "memory");
+    return r != 0;
+}
+
+// One block's share of a pair of tiles.
 struct Seg {
     int q0, n, len;        // the request
     int b, h, tok0;        // first token of the pair
@@ -156,8 +226,7 @@ struct Seg {
     int lo_tile, tiles;    // key tiles of the pair
     int k0, k1;            // this block's share of them
     int c[2];              // key tiles of each tile of rows in the share
-    int64_t u0;            // first unit of the pair
-    int units;
+    int first, last;       // blocks that share the pair
 };
 
 template <int D> struct Walk {
@@ -190,7 +259,7 @@ template <int D> struct Walk {
         : p(p), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
         if (u < ue) rq = load_request(p.a, b, bad);
     }
-    __device__ __forceinline__ bool next(Seg &s) {
+    __device__ __forceinline__ bool next(Seg &s, int64_t total, int grid) {
         if (u >= ue) return false;
         int lo, hi, t;
         for (;;) {  // the pair that holds unit u
@@ -206,14 +275,14 @@ template <int D> struct Walk {
         }
         s.q0 = rq.q0, s.n = rq.n, s.len = rq.len, s.b = b, s.lo = lo, s.hi = hi;
         s.h = (int)((u - before) / t);
-        s.u0 = before + (int64_t)s.h * t;
-        s.units = t;
+        const int64_t u0 = before + (int64_t)s.h * t;  // first unit of the pair
+        s.first = unit_block(total, u0, grid), s.last = unit_block(total, u0 + t - 1, grid);
         s.tok0 = qt * NT * p.tile_tok;
         s.lo_tile = lo / KT;
         s.tiles = (hi + KT - 1) / KT - s.lo_tile;
         if (hi <= lo) s.tiles = 0;
-        s.k0 = (int)(u - s.u0), s.k1 = (int)min((int64_t)t, ue - s.u0);
-        u = s.u0 + s.k1;
+        s.k0 = (int)(u - u0), s.k1 = (int)min((int64_t)t, ue - u0);
+        u = u0 + s.k1;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int t0 = s.tok0 + i * p.tile_tok, t1 = min(rq.n, t0 + p.tile_tok);
@@ -223,6 +292,25 @@ template <int D> struct Walk {
             s.c[i] = max(0, min(min(s.k1, s.tiles), own) - s.k0);
         }
         return true;
+    }
+};
+
+// Reader's side of the slots: a warp takes the next share and gives it back.
+struct Shares {
+    uint64_t *full, *empty;
+    const Seg *slots;
+    volatile int *abort;
+    int *err;
+    uint32_t i;
+    __device__ __forceinline__ const Seg *take() {  // null: no more
+        if (!wait_b(&full[i & 1], (i >> 1) & 1, abort, err, 39)) return nullptr;
+        const Seg *s = slots + (i & 1);
+        return s->n > 0 ? s : nullptr;
+    }
+    __device__ __forceinline__ void give(int lane) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[i & 1]);
+        i++;
     }
 };
 
@@ -237,7 +325,9 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *kv_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *kv_empty = kv_full + NB;
     uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_full = p_full + 2;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(o_full + 2);
+    uint64_t *seg_full = o_full + 2, *seg_empty = seg_full + 2;
+    Seg *segs = reinterpret_cast<Seg *>(smem + L::OFF_SEG);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + 2);
     volatile int *s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int *s_last = reinterpret_cast<volatile int *>(tmem_slot + 2);  // one a tile
     int64_t *s_sum = reinterpret_cast<int64_t *>(smem);  // before the first copy arrives there
@@ -246,11 +336,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (tid == 0) {
         for (int i = 0; i < NB; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
         mbar_init(q_full, 1), mbar_init(q_empty, 1);
-        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 4), mbar_init(&o_full[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&o_full[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 2 + 8 * NT);
         *s_abort = 0;
         fence_mbar_init();
     }
-    if (warp == 9) {
+    if (warp == MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
@@ -292,18 +383,18 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (s_sum[mid] > ub) run_hi = mid;
         else run = mid + 1;
     }
-    Walk<D> walk(p, ub, ue, run * per, run ? s_sum[run - 1] : 0);
-    Seg s;
+    const int64_t run_before = run ? s_sum[run - 1] : 0;
     fence_async_shared();
     __syncthreads();
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
-        if (warp == 8) {  // ---- TMA
+    Shares shares{seg_full, seg_empty, segs, s_abort, a.err, 0};
+    if (warp >= SOFT_WARPS) {
+        if (warp == TMA_WARP) {
             const int rows = p.box_rows, nrow = KT / rows, nbox = nrow * (D / 64);
             bool bad_page = false;
             uint32_t fills = 0, items = 0;
-            while (walk.next(s)) {
+            for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
+                const Seg s = *sp;
                 const int n = max(s.c[0], s.c[1]);
                 if (n == 0) continue;
                 wait_b(q_empty, (items & 1) ^ 1, s_abort, a.err, 31);
@@ -344,10 +435,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (*s_abort)  // nothing consumes what is still in flight: let it land before the block ends
                 for (uint32_t f = fills > NB ? fills - NB : 0; f < fills; f++)
                     mbar_wait(&kv_full[f % NB], (f / NB) & 1, 1u << 20);
-        } else if (warp == 9) {  // ---- MMA
+        } else if (warp == MMA_WARP) {
             constexpr uint32_t id_s = idesc<F16>(KT, false), id_o = idesc<F16>(D, true);
             uint32_t takes = 0, items = 0, np[2] = {0, 0}, ns = 0;
-            while (walk.next(s)) {
+            for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
+                const Seg s = *sp;
                 const int n = max(s.c[0], s.c[1]);
                 if (n == 0) continue;
                 wait_b(q_full, items & 1, s_abort, a.err, 33);
@@ -367,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         const uint32_t sv = smem_u32(smem + L::OFF_KV + (take % NB) * L::KV_BYTES);
 #pragma unroll
                         for (int kk = 0; kk < KT / 16; kk++)
-                            mma_ts(tmem + L::O_COL + t * D, tmem + L::S_COL + buf * KT + kk * 8, desc_mn(sv + kk * 2048), id_o,
+                            mma_ts(tmem + L::O_COL + t * D, tmem + L::S_COL + buf * KT + (kk >> 1) * 32 + (kk & 1) * 8, desc_mn(sv + kk * 2048), id_o,
                                    acc || kk ? 1u : 0u);
                     }
                     if (lane == 0) commit(&o_full[t]);
@@ -442,18 +534,34 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
                 takes += 2 * n;
             }
+        } else if (warp == WALK_WARP) {
+            Walk<D> walk(p, ub, ue, run * per, run_before);
+            Seg s;
+            for (uint32_t i = 0;; i++) {
+                const bool more = walk.next(s, total, grid);
+                if (!more) s.n = 0;
+                if (!wait_b(&seg_empty[i & 1], ((i >> 1) & 1) ^ 1, s_abort, a.err, 40)) break;
+                if (lane == 0) {
+                    segs[i & 1] = s;
+                    mbar_arrive(&seg_full[i & 1]);
+                }
+                if (!more) break;
+            }
         }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
-        // ---- softmax: this thread's row of tile t
-        const int t = warp >> 2, row = tid & 127;
+    } else if (NT == 2 || warp < 8) {
+        // softmax: thread (row, half) has 64 of the 128 keys of a row of tile t; the
+        // two threads of a row sit in warps w and w + 4, joined by a barrier of 64
+        const int t = warp >> 3, half = (warp >> 2) & 1, row = tid & 127, pair_bar = 1 + t * 4 + (warp & 3);
+        float *xch = reinterpret_cast<float *>(smem + L::OFF_X) + t * 2 * TM;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 * (warp % 4)
-        const uint32_t o_addr = tmem + lanes + L::O_COL + (NT == 2 ? t : 0) * D;
+        const uint32_t o_addr = tmem + lanes + L::O_COL + (NT == 2 ? t : 0) * D + half * (D / 2);
         const float sl2 = CAP ? 1.0f : a.scale * LOG2E;
         const float cap_in = CAP ? 2.0f * LOG2E * a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
         const float slack = 8.0f / sl2;  // the reference lags the maximum by up to 2^8
+        const uint64_t sl2_2 = pack2f(sl2, sl2);
         uint32_t nsf = 0, no = 0;        // S tiles and P V products of this tile so far
-        while (t < NT && walk.next(s)) {
+        for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
+            const volatile Seg &s = *sp;
             const int tok = s.tok0 + t * p.tile_tok + row / a.G;
             const int live_tok = min(s.n, s.tok0 + (t + 1) * p.tile_tok);
             const bool live = row < p.tile_tok * a.G && tok < live_tok;
@@ -462,74 +570,94 @@ __global__ void __launch_bounds__(THREADS, 1)
             // keys that every row of the tile sees
             const int all_hi = a.causal ? shift + s.tok0 + t * p.tile_tok : s.len, all_lo = a.window ? shift + live_tok - 1 - a.window : 0;
             float ref = -INFINITY, l = 0.f;
-            const int c = s.c[t];
+            const int c = s.c[t], first_key = (s.lo_tile + s.k0) * KT;
             for (int j = 0; j < c; j++) {
-                const int buf = NT == 2 ? t : (int)(nsf & 1), key0 = (s.lo_tile + s.k0 + j) * KT;
+                const int buf = NT == 2 ? t : (int)(nsf & 1), key0 = first_key + j * KT;
                 const uint32_t s_addr = tmem + lanes + L::S_COL + buf * KT;
                 wait_b(&s_full[buf], NT == 2 ? nsf & 1 : (nsf >> 1) & 1, s_abort, a.err, 36);
                 nsf++;
                 tc_after();
-                uint32_t x[KT];
-#pragma unroll
-                for (int i = 0; i < KT; i += 32) tmem_ld32(s_addr + i, x + i);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < KT; i++) pin(x[i]);
-                float *f = reinterpret_cast<float *>(x);
-                if (CAP) {
-#pragma unroll
-                    for (int i = 0; i < KT; i++) f[i] = soft_cap(f[i], cap_in, cap_out);
-                }
-                if (key0 + KT > all_hi || key0 < all_lo) {
-                    const int hi_i = lim - key0, lo_i = low - key0;
-#pragma unroll
-                    for (int i = 0; i < KT; i++) f[i] = i < hi_i && i >= lo_i ? f[i] : -INFINITY;
-                }
-                float m0 = f[0], m1 = f[1], m2 = f[2], m3 = f[3];
-#pragma unroll
-                for (int i = 4; i < KT; i += 4) {
-                    m0 = fmaxf(m0, f[i]), m1 = fmaxf(m1, f[i + 1]);
-                    m2 = fmaxf(m2, f[i + 2]), m3 = fmaxf(m3, f[i + 3]);
-                }
-                const float mx = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
-                // O and l are kept relative to `ref`, which follows the maximum only when
-                // that has outgrown it by 2^8: f32 holds the excess exactly, P's type too
-                const bool grow = j == 0 ? true : mx > ref + slack;
-                if (__any_sync(0xffffffffu, grow && j > 0)) {
-                    const float to = grow ? mx : ref;
-                    const float k = ref == -INFINITY ? (grow ? 0.f : 1.f) : ex2((ref - to) * sl2);
-                    l *= k;
-                    ref = to;
-                    wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 37);
-                    tc_after();
-#pragma unroll
-                    for (int d = 0; d < D; d += 32) {
-                        uint32_t o[32];
-                        tmem_ld32(o_addr + d, o);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            pin(o[i]);
-                            o[i] = __float_as_uint(__uint_as_float(o[i]) * k);
-                        }
-                        tmem_st32(o_addr + d, o);
-                    }
-                } else if (j == 0) ref = mx;
-                const float base = ref == -INFINITY ? 0.f : ref * sl2;
-                float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-                for (int g = 0; g < KT; g += 64) {
-                    uint32_t pk[32];
+                // S in two chunks of 32 keys: the second stays in registers, the first is read
+                // again for its exponentials (holding both would not leave enough registers)
+                uint32_t x[32];
+                auto load = [&](int chunk) {
+                    tmem_ld32(s_addr + half * HC + chunk * 32, x);
+                    tmem_wait_ld();
+                    const int k = key0 + half * HC + chunk * 32;
 #pragma unroll
                     for (int i = 0; i < 32; i++) {
-                        const float p0 = ex2(fmaf(f[g + 2 * i], sl2, -base)), p1 = ex2(fmaf(f[g + 2 * i + 1], sl2, -base));
-                        l0 += p0, l1 += p1;
+                        pin(x[i]);
+                        if (CAP) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), cap_in, cap_out));
+                    }
+                    if (key0 + KT > all_hi || key0 < all_lo) {
+#pragma unroll
+                        for (int i = 0; i < 32; i++) x[i] = k + i < lim && k + i >= low ? x[i] : 0xff800000u;
+                    }
+                };
+                auto largest = [&] {
+                    float m0 = max3f(x[0], x[1], x[2]), m1 = max3f(x[3], x[4], x[5]);
+#pragma unroll
+                    for (int i = 6; i < 30; i += 4) {
+                        m0 = max3f(__float_as_uint(m0), x[i], x[i + 1]);
+                        m1 = max3f(__float_as_uint(m1), x[i + 2], x[i + 3]);
+                    }
+                    return max3f(__float_as_uint(m0), __float_as_uint(m1), __float_as_uint(fmaxf(__uint_as_float(x[30]), __uint_as_float(x[31]))));
+                };
+                load(0);
+                float mx = largest();
+                load(1);
+                mx = fmaxf(mx, largest());
+                // O and l are kept relative to `ref`, which follows the maximum only when
+                // that has outgrown it by 2^8 (P's type and f32 both hold the excess), so
+                // the two threads of a row mostly need no more than this one vote
+                if (bar_or(pair_bar, j == 0 || mx > ref + slack)) {
+                    xch[half * TM + row] = mx;
+                    named_bar_sync(pair_bar, 64);
+                    mx = fmaxf(mx, xch[(half ^ 1) * TM + row]);
+                    if (j == 0) ref = mx;
+                    else {
+                        const float to = mx > ref + slack ? mx : ref;
+                        const float k = to == ref ? 1.0f : ex2((ref - to) * sl2);  // 0 when nothing was seen before
+                        l *= k;
+                        ref = to;
+                        wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 37);
+                        tc_after();
+#pragma unroll 1
+                        for (int d = 0; d < D / 2; d += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o_addr + d, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                pin(o[i]);
+                                o[i] = __float_as_uint(__uint_as_float(o[i]) * k);
+                            }
+                            tmem_st16(o_addr + d, o);
+                        }
+                    }
+                }
+                const float base = ref == -INFINITY ? 0.f : -ref * sl2;
+                const uint64_t base2 = pack2f(base, base);
+                uint64_t l2 = 0;
+#pragma unroll
+                for (int chunk = 1; chunk >= 0; chunk--) {
+                    if (chunk == 0) load(0);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        uint64_t y = fma2(pack2u(x[2 * i], x[2 * i + 1]), sl2_2, base2);
+                        y = i % 8 < POLY ? exp2_poly(y) : exp2_mufu(y);
+                        l2 = add2(l2, y);
                         // rounded to the values' type for the product; the sum stays in f32
+                        float p0, p1;
+                        unpack2f(y, p0, p1);
                         pk[i] = pack_half<F16>(p0, p1);
                     }
-                    tmem_st32(s_addr + g / 2, pk);
+                    tmem_st16(s_addr + half * HC + chunk * 32, pk);  // over the scores it came from
                 }
-                l += l0 + l1;
+                float la, lb;
+                unpack2f(l2, la, lb);
+                l += la + lb;
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();
@@ -537,20 +665,25 @@ __global__ void __launch_bounds__(THREADS, 1)
                 no++;
             }
             // ---- the tile's rows, or this block's part of them
-            const int first = unit_block(total, s.u0, grid), last = unit_block(total, s.u0 + s.units - 1, grid);
+            const int first = s.first, last = s.last;
             const bool has_tile = s.tok0 + t * p.tile_tok < s.n;
             if (!has_tile) continue;
+            named_bar_sync(pair_bar, 64);  // the last exchange is read
+            xch[half * TM + row] = l;
+            named_bar_sync(pair_bar, 64);
+            l += xch[(half ^ 1) * TM + row];
+            if (ref == -INFINITY) l = 0.f;  // no key seen (exp2_poly gives a masked one 2^-126)
             if (c > 0) {
                 wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 38);
                 tc_after();
             }
             const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row % a.G;
-            uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + orow * D;
+            uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + orow * D + half * (D / 2);
             const float ml = ref * sl2;  // log2 units
             if (first == last) {
                 const float inv = l > 0.f ? 1.0f / l : 0.f;
-#pragma unroll
-                for (int d = 0; d < D; d += 32) {
+#pragma unroll 1
+                for (int d = 0; d < D / 2; d += 32) {
                     uint32_t o[32];
                     if (c > 0) {
                         tmem_ld32(o_addr + d, o);
@@ -572,16 +705,16 @@ __global__ void __launch_bounds__(THREADS, 1)
                             *reinterpret_cast<uint4 *>(dst + d + i) = w;
                         }
                 }
-                if (live && a.lse) a.lse[orow] = l > 0.f ? ml * LN2 + logf(l) : -INFINITY;
+                if (live && half == 0 && a.lse) a.lse[orow] = l > 0.f ? ml * LN2 + logf(l) : -INFINITY;
                 continue;
             }
             // partial rows: m, l [128], then float4 [D / 4][128] (a warp's rows side by side)
             float *part = a.part + (int64_t)((blockIdx.x * 2 + (s.k0 == 0 ? 1 : 0)) * NT + t) * L::PART;
-            part[row] = l > 0.f ? ml : -INFINITY;
-            part[TM + row] = l;
+            if (half == 0) part[row] = l > 0.f ? ml : -INFINITY, part[TM + row] = l;
+            const int d0 = half * (D / 2);
             if (c > 0) {
-#pragma unroll
-                for (int d = 0; d < D; d += 32) {
+#pragma unroll 1
+                for (int d = 0; d < D / 2; d += 32) {
                     uint32_t o[32];
                     tmem_ld32(o_addr + d, o);
                     tmem_wait_ld();
@@ -589,19 +722,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int i = 0; i < 32; i++) pin(o[i]);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4 *>(part + 2 * TM + ((d + i) / 4 * TM + row) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<uint4 *>(part + 2 * TM + ((d0 + d + i) / 4 * TM + row) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
             }
             __threadfence();
-            named_bar_sync(1 + t, 128);
-            if (row == 0) {
+            named_bar_sync(9 + t, 256);
+            if (row == 0 && half == 0) {
                 const int n = atomicAdd(a.cnt + first * 2 + t, 1);
                 s_last[t] = n == last - first;
                 if (n == last - first) a.cnt[first * 2 + t] = 0;
             }
-            named_bar_sync(1 + t, 128);
+            named_bar_sync(9 + t, 256);
             const bool join = s_last[t];
-            named_bar_sync(1 + t, 128);  // s_last is read before the next tile's
+            named_bar_sync(9 + t, 256);  // s_last is read before the next tile's
             if (!join) continue;
             __threadfence();
             float mm = -INFINITY;
@@ -615,35 +748,35 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             const float inv = ll > 0.f ? 1.0f / ll : 0.f;
 #pragma unroll 1
-            for (int d = 0; d < D; d += 64) {
-                float4 acc[16];
+            for (int d = 0; d < D / 2; d += 32) {
+                float4 acc[8];
 #pragma unroll
-                for (int i = 0; i < 16; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
                 for (int b = first; b <= last; b++) {
                     const float *q = a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART;
                     const float mb = __ldcg(q + row);
                     if (mb == -INFINITY) continue;
                     const float w = ex2(mb - mm);
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(q + 2 * TM) + (d / 4 + i) * TM + row);
+                    for (int i = 0; i < 8; i++) {
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(q + 2 * TM) + ((d0 + d) / 4 + i) * TM + row);
                         acc[i].x += w * v.x, acc[i].y += w * v.y, acc[i].z += w * v.z, acc[i].w += w * v.w;
                     }
                 }
                 if (live)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2)
+                    for (int i = 0; i < 8; i += 2)
                         *reinterpret_cast<uint4 *>(dst + d + i * 4) =
                             make_uint4(pack_half<F16>(acc[i].x * inv, acc[i].y * inv), pack_half<F16>(acc[i].z * inv, acc[i].w * inv),
                                        pack_half<F16>(acc[i + 1].x * inv, acc[i + 1].y * inv), pack_half<F16>(acc[i + 1].z * inv, acc[i + 1].w * inv));
             }
-            if (live && a.lse) a.lse[orow] = ll > 0.f ? mm * LN2 + logf(ll) : -INFINITY;
+            if (live && half == 0 && a.lse) a.lse[orow] = ll > 0.f ? mm * LN2 + logf(ll) : -INFINITY;
         }
     }
     tc_before();
     __syncthreads();
     tc_after();
-    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
 bool encode(CUtensorMap *m, bool f16, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
