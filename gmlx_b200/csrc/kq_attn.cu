@@ -61,8 +61,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
     using L = RL<D>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t s_sum[NW * 32];
-    __shared__ int s_last;
+    __shared__ int64_t s_warp[NW], s_before;
+    __shared__ int s_run, s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     bool bad = false, bad_page = false;
 
@@ -73,24 +73,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
         const int b = tid * per + i;
         if (b < nb) mine += request_units(a, load_request(a, b, bad));
     }
-    s_sum[tid] = mine;
-    __syncthreads();
-    if (warp == 0) {
-        int64_t base = 0;
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            int64_t v = s_sum[w * 32 + lane];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
-            s_sum[w * 32 + lane] = v + base;
-            base += __shfl_sync(0xffffffffu, v, 31);
-        }
-    }
-    __syncthreads();
-    const int64_t total = s_sum[NW * 32 - 1];
+    int64_t total;
+    const int64_t upto = block_scan<NW * 32>(mine, s_warp, total);
     // at most one block a unit, so that the blocks of a row tile are neighbours
     const int grid = (int)min((int64_t)gridDim.x, total);
     if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
@@ -98,14 +82,10 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
     const int64_t ub = unit_begin(total, blockIdx.x, grid), ue = unit_begin(total, blockIdx.x + 1, grid);
 
     // the request that holds unit ub
-    int lo_t = 0, hi_t = NW * 32 - 1;
-    while (lo_t < hi_t) {
-        const int mid = (lo_t + hi_t) >> 1;
-        if (s_sum[mid] > ub) hi_t = mid;
-        else lo_t = mid + 1;
-    }
-    int b = lo_t * per;
-    int64_t before = lo_t ? s_sum[lo_t - 1] : 0;  // units before request b
+    if (upto - mine <= ub && ub < upto) s_run = tid, s_before = upto - mine;
+    __syncthreads();
+    int b = s_run * per;
+    int64_t before = s_before;  // units before request b
     Request rq = load_request(a, b, bad);
     for (;;) {
         const int64_t n = request_units(a, rq);
@@ -118,7 +98,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
     const uint16_t *kc = reinterpret_cast<const uint16_t *>(a.kc), *vc = reinterpret_cast<const uint16_t *>(a.vc);
     const int gr = lane >> 2, gc = lane & 3;
     const float sl2 = a.scale * LOG2E;
-    const float cap_in = a.softcap > 0.f ? 2.0f * LOG2E * a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
+    const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
 
     for (int64_t u = ub; u < ue;) {
         int64_t units = request_units(a, rq);

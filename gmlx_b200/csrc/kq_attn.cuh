@@ -47,11 +47,38 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// cap * tanh(z / cap) in units of log2, from one exponential and one reciprocal:
-// tanh(u) = 1 - 2 / (1 + e^2u) (the hardware's tanh is good to 11 bits only,
-// too few for a score of up to `cap`)
-__device__ __forceinline__ float soft_cap(float x, float in2, float out) {
-    return out - __fdividef(2.0f * out, 1.0f + ex2(x * in2));
+// softcap in units of log2: out * tanh(x * in), with 1 - 2 / (1 + e^2u) for the
+// tanh (the hardware's is good to 11 bits only, too few for a score of up to `cap`)
+__device__ __forceinline__ float soft_cap(float x, float in, float out) {
+    return out - __fdividef(2.0f * out, 1.0f + ex2(x * (2.0f * LOG2E * in)));
+}
+
+// Where a block's run of units starts, when thread i of it counted `mine` units
+// in its run of requests: that thread and the units before it; the units in all.
+struct Start {
+    int thread;
+    int64_t before, total;
+};
+template <int N> __device__ __forceinline__ int64_t block_scan(int64_t mine, int64_t *s_warp, int64_t &total) {  // inclusive
+    static_assert(N % 32 == 0 && N <= 1024, "whole warps");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t v = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) s_warp[warp] = v;
+    __syncthreads();
+    int64_t w = lane < N / 32 ? s_warp[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t u = __shfl_up_sync(0xffffffffu, w, o);
+        if (lane >= o) w += u;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const int64_t below = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    return v + (warp ? below : 0);
 }
 
 // Unit u of `total` belongs to block ((u + 1) * grid - 1) / total, when block c

@@ -15,12 +15,15 @@
 // Blocks are persistent, one an SM.  The units of work (128 keys of one pair of
 // tiles) stand in one line over all requests and every block takes an equal run
 // of them; what a run cuts off goes through f32 partial rows in the workspace,
-// joined by the last block to arrive, in block order.
+// which a second small launch joins in block order.  When there is a block for
+// every pair and the longest pair takes little longer than an equal run (a short
+// prompt), blocks take whole pairs instead.
 //
-// Warps 0-7 and 8-15: softmax of tile 0 and 1, and their results; warp 16: TMA of
-// queries and pages (a page's rows of one head and 64 values a box; boxes that
-// no row sees are read out of bounds, which fills zeros); warp 17: MMA issue;
-// warp 18: walks the block's run of units and hands its shares of tile pairs to
+// Warps 0-7 and 8-15: softmax of tile 0 and 1, and their results; warps 16 and 19:
+// TMA of queries and keys, and of values (a page's rows of one head and 64 values
+// a box; boxes that no row sees are read out of bounds, which fills zeros; two
+// warps, since a 16-token page makes 16 boxes a tile at some 50 clocks each);
+// warp 17: MMA issue; warp 18: walks the block's run of units and hands its shares of tile pairs to
 // the others through two slots in shared memory (their registers hold scores).
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -33,7 +36,7 @@ namespace kq {
 namespace {
 
 constexpr int TM = 128, KT = 128;  // rows a tile, keys a unit
-constexpr int SOFT_WARPS = 16, TMA_WARP = 16, MMA_WARP = 17, WALK_WARP = 18, THREADS = 640;
+constexpr int SOFT_WARPS = 16, K_WARP = 16, MMA_WARP = 17, WALK_WARP = 18, V_WARP = 19, THREADS = 640;
 constexpr int HC = KT / 2;  // keys of a row that one thread handles
 
 template <int D> struct TL {
@@ -50,10 +53,18 @@ template <int D> struct TL {
 
 struct TileArgs {
     AttnArgs a;
-    int box_rows;    // rows of a page box
+    int box_shift;   // log2 of a page box's rows
     int tile_tok;    // tokens a tile: 128 / G
     uint32_t q_tx;   // bytes of a tile's queries
+    int whole;       // blocks may take whole pairs (their number fits 32 bits)
 };
+
+// What the join needs of a pair that block `i` begins and others end; last == i: none.
+struct Split {
+    int last, q0, n, tok0, h;
+};
+constexpr int SPLIT_FLOATS = 8 * 256;  // room for one a block in front of the partial rows
+constexpr int JOIN_COST = 2;           // what a cut costs, in units: rows written, and the join's launch
 
 __device__ __forceinline__ uint64_t gtimer() {
     uint64_t t;
@@ -175,6 +186,11 @@ __device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
     return v;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+    uint64_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(x), "l"(y));
+    return v;
+}
 __device__ __forceinline__ float max3f(uint32_t x, uint32_t y, uint32_t z) {
     float v;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(__uint_as_float(x)), "f"(__uint_as_float(y)), "f"(__uint_as_float(z)));
@@ -208,6 +224,33 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
     return pack2u(__float_as_uint(y0) + (__float_as_uint(n0) << 23), __float_as_uint(y1) + (__float_as_uint(n1) << 23));
 }
 
+// Capped scores in units of log2.  While |x * in| <= 1 for all of a warp's (a score
+// within the cap: as good as always) the tanh is an odd polynomial, whose largest
+// relative error on that interval is smallest (6.7e-7), and leaves the SFU alone.
+__device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) m = max3f(__float_as_uint(m), x[i] & 0x7fffffffu, x[i + 1] & 0x7fffffffu);
+    if (__all_sync(0xffffffffu, m * in <= 1.0f)) {
+        const float c[6] = {0.9999994039535522f, -0.3332904279232025f, 0.13281433284282684f,
+                            -0.051605675369501114f, 0.016743114218115807f, -0.003067060373723507f};
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            const uint64_t u = mul2(pack2u(x[i], x[i + 1]), pack2f(in, in)), v = mul2(u, u);
+            uint64_t y = fma2(v, pack2f(c[5], c[5]), pack2f(c[4], c[4]));
+#pragma unroll
+            for (int k = 3; k >= 0; k--) y = fma2(y, v, pack2f(c[k], c[k]));
+            y = mul2(mul2(y, u), pack2f(out, out));
+            float a, b;
+            unpack2f(y, a, b);
+            x[i] = __float_as_uint(a), x[i + 1] = __float_as_uint(b);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), in, out));
+    }
+}
+
 // Barrier of a warp pair (64 threads) that gives the OR of their predicates.
 __device__ __forceinline__ bool bar_or(int id, bool v) {
     uint32_t r;
@@ -232,6 +275,7 @@ struct Seg {
 template <int D> struct Walk {
     static constexpr int NT = TL<D>::NT;
     const TileArgs &p;
+    bool whole;  // a pair is one unit
     int64_t u, ue, before;
     Request rq;
     int b, qt;  // request, pair
@@ -247,16 +291,22 @@ template <int D> struct Walk {
         if (rows == 0 || rows > p.a.max_rows || rows < p.a.min_rows) return 0;
         return (r.n + NT * p.tile_tok - 1) / (NT * p.tile_tok);
     }
-    __device__ __forceinline__ static int64_t request_units(const TileArgs &p, const Request &r) {
+    // units and pairs of a request; `most`: the longest pair so far
+    __device__ __forceinline__ static int64_t request_units(const TileArgs &p, const Request &r, int64_t &items, int &most) {
         const int n = pairs(p, r);
         int64_t s = 0;
         int lo, hi;
-        for (int i = 0; i < n; i++) s += pair_units(p, r, i, lo, hi);
+        for (int i = 0; i < n; i++) {
+            const int t = pair_units(p, r, i, lo, hi);
+            s += t;
+            most = max(most, t);
+        }
+        items += (int64_t)n * p.a.Hk;
         return s * p.a.Hk;
     }
 
-    __device__ __forceinline__ Walk(const TileArgs &p, int64_t ub, int64_t ue, int b0, int64_t before0)
-        : p(p), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
+    __device__ __forceinline__ Walk(const TileArgs &p, bool whole, int64_t ub, int64_t ue, int b0, int64_t before0)
+        : p(p), whole(whole), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
         if (u < ue) rq = load_request(p.a, b, bad);
     }
     __device__ __forceinline__ bool next(Seg &s, int64_t total, int grid) {
@@ -265,6 +315,7 @@ template <int D> struct Walk {
         for (;;) {  // the pair that holds unit u
             if (qt < pairs(p, rq)) {
                 t = pair_units(p, rq, qt, lo, hi);
+                if (whole) t = 1;
                 if (u < before + (int64_t)t * p.a.Hk) break;
                 before += (int64_t)t * p.a.Hk;
                 qt++;
@@ -283,6 +334,7 @@ template <int D> struct Walk {
         if (hi <= lo) s.tiles = 0;
         s.k0 = (int)(u - u0), s.k1 = (int)min((int64_t)t, ue - u0);
         u = u0 + s.k1;
+        if (whole) s.k1 = max(1, s.tiles);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int t0 = s.tok0 + i * p.tile_tok, t1 = min(rq.n, t0 + p.tile_tok);
@@ -314,6 +366,12 @@ struct Shares {
     }
 };
 
+// Partial rows of a tile that block `blk` cut: its last pair when it begins the
+// pair, else its first.
+template <int D> __device__ __forceinline__ float *part_of(float *base, int blk, bool begins, int t) {
+    return base + SPLIT_FLOATS + (int64_t)((blk * 2 + (begins ? 1 : 0)) * TL<D>::NT + t) * TL<D>::PART;
+}
+
 template <bool F16, int D, bool CAP>
 __global__ void __launch_bounds__(THREADS, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -329,15 +387,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     Seg *segs = reinterpret_cast<Seg *>(smem + L::OFF_SEG);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + 2);
     volatile int *s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    volatile int *s_last = reinterpret_cast<volatile int *>(tmem_slot + 2);  // one a tile
-    int64_t *s_sum = reinterpret_cast<int64_t *>(smem);  // before the first copy arrives there
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     if (tid == 0) {
         for (int i = 0; i < NB; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
         mbar_init(q_full, 1), mbar_init(q_empty, 1);
         for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&o_full[i], 1);
-        for (int i = 0; i < 2; i++) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 2 + 8 * NT);
+        for (int i = 0; i < 2; i++) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 3 + 8 * NT);
         *s_abort = 0;
         fence_mbar_init();
     }
@@ -348,92 +404,102 @@ __global__ void __launch_bounds__(THREADS, 1)
     // units of each thread's run of requests (b == B: the padding tokens)
     bool bad = false;
     const int nb = a.B + 1, per = (nb + THREADS - 1) / THREADS;
-    int64_t mine = 0;
+    int64_t mine = 0, items = 0;
+    int most = 0;
     for (int i = 0; i < per; i++) {
         const int b = tid * per + i;
-        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad));
+        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad), items, most);
     }
-    s_sum[tid] = mine;
+    Split *splits = reinterpret_cast<Split *>(a.part);
+    if (tid == 0) splits[blockIdx.x].last = blockIdx.x;
     if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
+    int64_t *s_warp = reinterpret_cast<int64_t *>(smem);  // before the first copy arrives there
+    int *s_most = reinterpret_cast<int *>(s_warp + 64), *s_run = s_most + 32;
+    int64_t *s_before = s_warp + 96;
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) s_most[warp] = most;
+    int64_t total, pairs;
+    int64_t upto = block_scan<THREADS>(mine, s_warp, total);
+    const int64_t items_upto = block_scan<THREADS>(items, s_warp + 32, pairs);
+    most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s_most[lane] : 0);
+    const bool whole = p.whole && pairs <= gridDim.x && most <= (total + gridDim.x - 1) / gridDim.x + JOIN_COST;
+    if (whole) total = pairs, upto = items_upto, mine = items;
+    const int grid = (int)min((int64_t)gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
+    const bool work = (int)blockIdx.x < grid;
+    const int64_t ub = work ? unit_begin(total, blockIdx.x, grid) : 0, ue = work ? unit_begin(total, blockIdx.x + 1, grid) : 0;
+    if (work && upto - mine <= ub && ub < upto) *s_run = tid, *s_before = upto - mine;
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = *tmem_slot;
-    if (warp == 0) {
-        int64_t base = 0;
-        for (int w = 0; w < THREADS / 32; w++) {
-            int64_t v = s_sum[w * 32 + lane];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t x = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += x;
-            }
-            s_sum[w * 32 + lane] = v + base;
-            base += __shfl_sync(0xffffffffu, v, 31);
-        }
-    }
-    __syncthreads();
-    const int64_t total = s_sum[THREADS - 1];
-    const int grid = (int)min((int64_t)gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
-    const bool work = (int)blockIdx.x < grid;
-    const int64_t ub = work ? unit_begin(total, blockIdx.x, grid) : 0, ue = work ? unit_begin(total, blockIdx.x + 1, grid) : 0;
-    int run = 0, run_hi = THREADS - 1;
-    while (run < run_hi) {
-        const int mid = (run + run_hi) >> 1;
-        if (s_sum[mid] > ub) run_hi = mid;
-        else run = mid + 1;
-    }
-    const int64_t run_before = run ? s_sum[run - 1] : 0;
+    const int run = work ? *s_run : 0;
+    const int64_t run_before = work ? *s_before : 0;
     fence_async_shared();
     __syncthreads();
 
     Shares shares{seg_full, seg_empty, segs, s_abort, a.err, 0};
     if (warp >= SOFT_WARPS) {
-        if (warp == TMA_WARP) {
-            const int rows = p.box_rows, nrow = KT / rows, nbox = nrow * (D / 64);
+        if (warp == K_WARP || warp == V_WARP) {
+            // box r of a tile: keys [r << shift, (r + 1) << shift) of one page, for each
+            // 64 values of the head; the pages of the next tile are looked up while
+            // this one waits for its place in the ring
+            const int kv = warp == V_WARP, shift = p.box_shift, nrow = KT >> shift;
+            const CUtensorMap *map = kv ? &tm_v : &tm_k;
             bool bad_page = false;
-            uint32_t fills = 0, items = 0;
+            uint32_t fill = kv, items = 0;  // keys take the even fills of the ring, values the odd ones
             for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
-                const Seg s = *sp;
-                const int n = max(s.c[0], s.c[1]);
+                const int n = max(sp->c[0], sp->c[1]), h = sp->h, lo = sp->lo, hi = sp->hi, key00 = (sp->lo_tile + sp->k0) * KT;
                 if (n == 0) continue;
-                wait_b(q_empty, (items & 1) ^ 1, s_abort, a.err, 31);
-                items++;
-                if (lane == 0) {
-                    const int live = s.c[NT - 1] > 0 ? NT : 1;
-                    mbar_arrive_expect_tx(q_full, live * p.q_tx);
-                    if (!*s_abort)
-                        for (int t = 0; t < live; t++)
-                            for (int d = 0; d < D / 64; d++)
-                                tma_3d(smem + t * L::Q_BYTES + d * TM * 128, &tm_q, d * 64, s.h * a.G, s.q0 + s.tok0 + t * p.tile_tok, q_full);
-                }
-                const int32_t *bt = a.table + (int64_t)s.b * a.table_stride;
-                for (int j = 0; j < n; j++) {
-                    const int tile0 = (s.lo_tile + s.k0 + j) * KT;
-                    for (int kv = 0; kv < 2; kv++, fills++) {
-                        const int slot = fills % NB;
-                        wait_b(&kv_empty[slot], ((fills / NB) & 1) ^ 1, s_abort, a.err, 32);
-                        if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], L::KV_BYTES);
-                        __syncwarp();
-                        if (*s_abort) continue;
-                        for (int i = lane; i < nbox; i += 32) {
-                            const int r = i % nrow, d = i / nrow, key = tile0 + r * rows;
-                            int page = a.n_pages, col = 0;  // out of bounds: zeros
-                            if (key < s.hi && key + rows > s.lo) {
-                                col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
-                                const int id = bt[col];
-                                if ((unsigned)id < (unsigned)a.n_pages) page = id;
-                                else bad_page = true;
-                            }
-                            tma_4d(smem + L::OFF_KV + slot * L::KV_BYTES + d * KT * 128 + r * rows * 128, kv ? &tm_v : &tm_k, d * 64,
-                                   key - col * a.page < a.page ? max(0, key - col * a.page) : 0, s.h, page, &kv_full[slot]);
+                const int32_t *bt = a.table + (int64_t)sp->b * a.table_stride;
+                int page[4], off[4];
+                auto look_up = [&](int j) {
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int r = lane + 32 * q, key = key00 + j * KT + (r << shift);
+                        page[q] = a.n_pages, off[q] = 0;  // out of bounds: zeros
+                        if (r < nrow && key < hi && key + (1 << shift) > lo) {
+                            const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
+                            const int id = bt[col];
+                            off[q] = key - col * a.page;
+                            if ((unsigned)id < (unsigned)a.n_pages) page[q] = id;
+                            else bad_page = true;
                         }
                     }
+                };
+                look_up(0);
+                if (!kv) {
+                    wait_b(q_empty, (items & 1) ^ 1, s_abort, a.err, 31);
+                    items++;
+                    if (lane == 0) {
+                        const int live = sp->c[NT - 1] > 0 ? NT : 1;
+                        mbar_arrive_expect_tx(q_full, live * p.q_tx);
+                        if (!*s_abort)
+                            for (int t = 0; t < live; t++)
+#pragma unroll
+                                for (int d = 0; d < D / 64; d++)
+                                    tma_3d(smem + t * L::Q_BYTES + d * TM * 128, &tm_q, d * 64, h * a.G, sp->q0 + sp->tok0 + t * p.tile_tok, q_full);
+                    }
+                }
+                for (int j = 0; j < n; j++, fill += 2) {
+                    const int slot = fill % NB;
+                    uint8_t *dst = smem + L::OFF_KV + slot * L::KV_BYTES;
+                    const bool ok = wait_b(&kv_empty[slot], ((fill / NB) & 1) ^ 1, s_abort, a.err, 32);
+                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], L::KV_BYTES);
+                    __syncwarp();
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const int r = lane + 32 * q;
+                        if (r < nrow && ok)
+#pragma unroll
+                            for (int d = 0; d < D / 64; d++)
+                                tma_4d(dst + d * KT * 128 + (r << shift) * 128, map, d * 64, off[q], h, page[q], &kv_full[slot]);
+                    }
+                    if (j + 1 < n) look_up(j + 1);
                 }
             }
             if (bad_page) atomicCAS(a.err, 0, ERR_INDEX);
             if (*s_abort)  // nothing consumes what is still in flight: let it land before the block ends
-                for (uint32_t f = fills > NB ? fills - NB : 0; f < fills; f++)
+                for (uint32_t f = fill >= 2 * NB + kv ? fill - 2 * NB : kv; f < fill; f += 2)
                     mbar_wait(&kv_full[f % NB], (f / NB) & 1, 1u << 20);
         } else if (warp == MMA_WARP) {
             constexpr uint32_t id_s = idesc<F16>(KT, false), id_o = idesc<F16>(D, true);
@@ -535,7 +601,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 takes += 2 * n;
             }
         } else if (warp == WALK_WARP) {
-            Walk<D> walk(p, ub, ue, run * per, run_before);
+            Walk<D> walk(p, whole, ub, ue, run * per, run_before);
             Seg s;
             for (uint32_t i = 0;; i++) {
                 const bool more = walk.next(s, total, grid);
@@ -556,7 +622,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 * (warp % 4)
         const uint32_t o_addr = tmem + lanes + L::O_COL + (NT == 2 ? t : 0) * D + half * (D / 2);
         const float sl2 = CAP ? 1.0f : a.scale * LOG2E;
-        const float cap_in = CAP ? 2.0f * LOG2E * a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
+        const float cap_in = CAP ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
         const float slack = 8.0f / sl2;  // the reference lags the maximum by up to 2^8
         const uint64_t sl2_2 = pack2f(sl2, sl2);
         uint32_t nsf = 0, no = 0;        // S tiles and P V products of this tile so far
@@ -580,18 +646,22 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // S in two chunks of 32 keys: the second stays in registers, the first is read
                 // again for its exponentials (holding both would not leave enough registers)
                 uint32_t x[32];
-                auto load = [&](int chunk) {
+                auto load = [&](int chunk, bool again) {
                     tmem_ld32(s_addr + half * HC + chunk * 32, x);
                     tmem_wait_ld();
                     const int k = key0 + half * HC + chunk * 32;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        pin(x[i]);
-                        if (CAP) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), cap_in, cap_out));
-                    }
+                    for (int i = 0; i < 32; i++) pin(x[i]);
+                    if (CAP && again) return;
+                    if (CAP) cap_scores(x, cap_in, cap_out);
                     if (key0 + KT > all_hi || key0 < all_lo) {
 #pragma unroll
                         for (int i = 0; i < 32; i++) x[i] = k + i < lim && k + i >= low ? x[i] : 0xff800000u;
+                    }
+                    if (CAP && chunk == 0) {  // what is read again
+                        tmem_st16(s_addr + half * HC, x);
+                        tmem_st16(s_addr + half * HC + 16, x + 16);
+                        tmem_wait_st();
                     }
                 };
                 auto largest = [&] {
@@ -603,9 +673,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     return max3f(__float_as_uint(m0), __float_as_uint(m1), __float_as_uint(fmaxf(__uint_as_float(x[30]), __uint_as_float(x[31]))));
                 };
-                load(0);
+                load(0, false);
                 float mx = largest();
-                load(1);
+                load(1, false);
                 mx = fmaxf(mx, largest());
                 // O and l are kept relative to `ref`, which follows the maximum only when
                 // that has outgrown it by 2^8 (P's type and f32 both hold the excess), so
@@ -641,7 +711,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 uint64_t l2 = 0;
 #pragma unroll
                 for (int chunk = 1; chunk >= 0; chunk--) {
-                    if (chunk == 0) load(0);
+                    if (chunk == 0) load(0, true);
                     uint32_t pk[16];
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -709,9 +779,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 continue;
             }
             // partial rows: m, l [128], then float4 [D / 4][128] (a warp's rows side by side)
-            float *part = a.part + (int64_t)((blockIdx.x * 2 + (s.k0 == 0 ? 1 : 0)) * NT + t) * L::PART;
+            float *part = part_of<D>(a.part, blockIdx.x, s.k0 == 0, t);
             if (half == 0) part[row] = l > 0.f ? ml : -INFINITY, part[TM + row] = l;
-            const int d0 = half * (D / 2);
+            if (tid == 0 && s.k0 == 0) splits[blockIdx.x] = Split{last, s.q0, s.n, s.tok0, s.h};
             if (c > 0) {
 #pragma unroll 1
                 for (int d = 0; d < D / 2; d += 32) {
@@ -720,63 +790,57 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tmem_wait_ld();
 #pragma unroll
                     for (int i = 0; i < 32; i++) pin(o[i]);
+                    if (live)
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4 *>(part + 2 * TM + ((d0 + d + i) / 4 * TM + row) * 4) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4 *>(part + 2 * TM + ((half * (D / 2) + d + i) / 4 * TM + row) * 4) =
+                                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
             }
-            __threadfence();
-            named_bar_sync(9 + t, 256);
-            if (row == 0 && half == 0) {
-                const int n = atomicAdd(a.cnt + first * 2 + t, 1);
-                s_last[t] = n == last - first;
-                if (n == last - first) a.cnt[first * 2 + t] = 0;
-            }
-            named_bar_sync(9 + t, 256);
-            const bool join = s_last[t];
-            named_bar_sync(9 + t, 256);  // s_last is read before the next tile's
-            if (!join) continue;
-            __threadfence();
-            float mm = -INFINITY;
-            for (int b = first; b <= last; b++)
-                mm = fmaxf(mm, __ldcg(a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART + row));
-            float ll = 0.f;
-            for (int b = first; b <= last; b++) {
-                const float *q = a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART;
-                const float mb = __ldcg(q + row);
-                ll += mb == -INFINITY ? 0.f : ex2(mb - mm) * __ldcg(q + TM + row);
-            }
-            const float inv = ll > 0.f ? 1.0f / ll : 0.f;
-#pragma unroll 1
-            for (int d = 0; d < D / 2; d += 32) {
-                float4 acc[8];
-#pragma unroll
-                for (int i = 0; i < 8; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                for (int b = first; b <= last; b++) {
-                    const float *q = a.part + (int64_t)((b * 2 + (b == first ? 1 : 0)) * NT + t) * L::PART;
-                    const float mb = __ldcg(q + row);
-                    if (mb == -INFINITY) continue;
-                    const float w = ex2(mb - mm);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(q + 2 * TM) + ((d0 + d) / 4 + i) * TM + row);
-                        acc[i].x += w * v.x, acc[i].y += w * v.y, acc[i].z += w * v.z, acc[i].w += w * v.w;
-                    }
-                }
-                if (live)
-#pragma unroll
-                    for (int i = 0; i < 8; i += 2)
-                        *reinterpret_cast<uint4 *>(dst + d + i * 4) =
-                            make_uint4(pack_half<F16>(acc[i].x * inv, acc[i].y * inv), pack_half<F16>(acc[i].z * inv, acc[i].w * inv),
-                                       pack_half<F16>(acc[i + 1].x * inv, acc[i + 1].y * inv), pack_half<F16>(acc[i + 1].z * inv, acc[i + 1].w * inv));
-            }
-            if (live && half == 0 && a.lse) a.lse[orow] = ll > 0.f ? mm * LN2 + logf(ll) : -INFINITY;
         }
     }
     tc_before();
     __syncthreads();
     tc_after();
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
+// Joins the pair that block blockIdx.x of the tiles began and others ended: 32 of
+// its rows (blockIdx.y), a lane a row, each warp every eighth float4 of them.
+constexpr int JOIN_ROWS = 32, JOIN_WARPS = 8;
+template <bool F16, int D> __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ TileArgs p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const AttnArgs &a = p.a;
+    const int first = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Split s = reinterpret_cast<const Split *>(a.part)[first];
+    if (s.last == first) return;
+    const int t = blockIdx.y * JOIN_ROWS / TM, row = blockIdx.y * JOIN_ROWS % TM + lane;
+    const int tok = s.tok0 + t * p.tile_tok + row / a.G;
+    if (row >= p.tile_tok * a.G || tok >= min(s.n, s.tok0 + (t + 1) * p.tile_tok)) return;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 4
+    for (int b = first; b <= s.last; b++) m = fmaxf(m, part_of<D>(a.part, b, b == first, t)[row]);
+    float4 acc[D / 4 / JOIN_WARPS];
+#pragma unroll
+    for (int i = 0; i < D / 4 / JOIN_WARPS; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+    for (int b = first; b <= s.last; b++) {
+        const float *q = part_of<D>(a.part, b, b == first, t);
+        const float mb = q[row], w = mb == -INFINITY ? 0.f : ex2(mb - m);
+        l += w * q[TM + row];
+#pragma unroll
+        for (int i = 0; i < D / 4 / JOIN_WARPS; i++) {
+            const float4 v = reinterpret_cast<const float4 *>(q + 2 * TM)[(warp + i * JOIN_WARPS) * TM + row];
+            if (w != 0.f) acc[i].x += w * v.x, acc[i].y += w * v.y, acc[i].z += w * v.z, acc[i].w += w * v.w;
+        }
+    }
+    const float inv = l > 0.f ? 1.0f / l : 0.f;
+    const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row % a.G;
+#pragma unroll
+    for (int i = 0; i < D / 4 / JOIN_WARPS; i++)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + (warp + i * JOIN_WARPS) * 4) =
+            make_uint2(pack_half<F16>(acc[i].x * inv, acc[i].y * inv), pack_half<F16>(acc[i].z * inv, acc[i].w * inv));
+    if (warp == 0 && a.lse) a.lse[orow] = l > 0.f ? m * LN2 + logf(l) : -INFINITY;
 }
 
 bool encode(CUtensorMap *m, bool f16, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
@@ -790,11 +854,12 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     using L = TL<D>;
     TileArgs p;
     p.a = a;
-    int rows = 1;  // the largest power of two that divides both a page and a tile
-    while (rows < KT && a.page % (rows * 2) == 0) rows *= 2;
-    p.box_rows = rows;
+    int shift = 0;  // the largest power of two that divides both a page and a tile
+    while ((1 << shift) < KT && a.page % (2 << shift) == 0) shift++;
+    p.box_shift = shift;
     p.tile_tok = TM / a.G;
     p.q_tx = (uint32_t)(p.tile_tok * a.G * D * 2);
+    p.whole = (int64_t)a.T * a.Hk < (1ll << 30);
     CUtensorMap mq, mk, mv;
     // a dimension of one entry has no stride of its own
     auto bytes = [](int64_t s) { return (cuuint64_t)(s > 0 ? s * 2 : 16); };
@@ -802,13 +867,23 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     const cuuint32_t qb[3] = {64, (cuuint32_t)a.G, (cuuint32_t)p.tile_tok};
     const cuuint64_t cd[4] = {(cuuint64_t)D, (cuuint64_t)a.page, (cuuint64_t)a.Hk, (cuuint64_t)a.n_pages};
     const cuuint64_t cs[3] = {bytes(a.row_stride), bytes(a.head_stride), bytes(a.page_stride)};
-    const cuuint32_t cb[4] = {64, (cuuint32_t)rows, 1, 1};
+    const cuuint32_t cb[4] = {64, 1u << shift, 1, 1};
     taken = encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
     if (!taken) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<F16, D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
     if (e != cudaSuccess) return e;
     tiles_kernel<F16, D, CAP><<<num_sms(), THREADS, L::SMEM, st>>>(mq, mk, mv, p);
-    return cudaGetLastError();
+    // the join's launch overlaps the tiles' end
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(num_sms(), L::NT * TM / JOIN_ROWS);
+    cfg.blockDim = dim3(JOIN_WARPS * 32);
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<F16, D>, p);
 }
 
 template <bool F16, int D> cudaError_t launch_cap(const AttnArgs &a, cudaStream_t st, bool &taken) {
@@ -818,7 +893,7 @@ template <bool F16, int D> cudaError_t launch_cap(const AttnArgs &a, cudaStream_
 }  // namespace
 
 size_t attn_tiles_part_bytes(int D) {
-    return (size_t)num_sms() * 2 * (D <= 128 ? 2 : 1) * TM * (D + 2) * sizeof(float);
+    return ((size_t)num_sms() * 2 * (D <= 128 ? 2 : 1) * TM * (D + 2) + SPLIT_FLOATS) * sizeof(float);
 }
 
 cudaError_t launch_attn_tiles(const AttnArgs &a, int dtype, cudaStream_t st, bool &taken) {
