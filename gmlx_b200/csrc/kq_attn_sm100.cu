@@ -2,15 +2,16 @@
 // the 5th-generation tensor cores (tcgen05, accumulators in TMEM).
 //
 // A tile is 128 packed rows of one request and kv head (tokens x the query heads
-// that share the kv head); scores S = Q K^T of 128 keys at a time go to TMEM,
-// eight warps turn them into probabilities P, two threads a row with 64 keys
-// each (no shuffles), P goes back to TMEM over S and feeds O += P V, which stays
-// in TMEM.
+// that share the kv head); scores S = Q K^T go to TMEM, eight warps turn them into
+// probabilities P, sixteen rows each, P goes back to TMEM over S and feeds O += P V,
+// which stays in TMEM.
 //
-//   head dim 64, 128: two tiles a block, each with its own warps, S and O: the
-//     tensor core works on one tile while the other's softmax runs;
-//   head dim 256: O takes half of TMEM, so one tile a block with two S buffers:
-//     the tensor core computes the next S and the last P V meanwhile.
+// What bounds it: the products (a 128 x 128 x 16 step takes 64 clocks, and so does
+// one of half its width) and nearly as much time in exponentials (16 a clock and
+// SM).  One tile's scores, softmax and product are a chain, so a block works on two
+// tiles (head dim 64, 128; S of 128 keys each): the tensor core has the one while
+// the other's softmax runs.  At 256 O takes half of TMEM, so there is one tile, and
+// two S buffers of 64 keys.
 //
 // Blocks are persistent, one an SM.  The units of work (128 keys of one pair of
 // tiles) stand in one line over all requests and every block takes an equal run
@@ -22,9 +23,11 @@
 // Warps 0-7 and 8-15: softmax of tile 0 and 1, and their results; warps 16 and 19:
 // TMA of queries and keys, and of values (a page's rows of one head and 64 values
 // a box; boxes that no row sees are read out of bounds, which fills zeros; two
-// warps, since a 16-token page makes 16 boxes a tile at some 50 clocks each);
-// warp 17: MMA issue; warp 18: walks the block's run of units and hands its shares of tile pairs to
-// the others through two slots in shared memory (their registers hold scores).
+// warps, since a 16-token page makes 16 boxes a tile at some 50 clocks each); warp
+// 16 also walks the block's run of units and hands its shares of tile pairs to the
+// others through slots in shared memory.  Warps 17 and 18 issue the products of
+// tile 0 and 1: the queue to the tensor core is short and a thread's waits and
+// commits take some 500 clocks a step, which the other warp's products cover.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -36,18 +39,22 @@ namespace kq {
 namespace {
 
 constexpr int TM = 128, KT = 128;  // rows a tile, keys a unit
-constexpr int SOFT_WARPS = 16, K_WARP = 16, MMA_WARP = 17, WALK_WARP = 18, V_WARP = 19, THREADS = 640;
-constexpr int HC = KT / 2;  // keys of a row that one thread handles
+constexpr int SOFT_WARPS = 16, K_WARP = 16, MMA_WARP = 17, V_WARP = 19, THREADS = 640;  // MMA_WARP + t: tile t
+// 512 x 104 + 128 x 64 = 640 x 96 registers, what the launch holds
+constexpr int SOFT_REGS = 104, OTHER_REGS = 64;
+static_assert(SOFT_WARPS * 32 * SOFT_REGS + (THREADS - SOFT_WARPS * 32) * OTHER_REGS <= THREADS * 96, "register split");
 
 template <int D> struct TL {
     static constexpr int NT = D <= 128 ? 2 : 1;
-    static constexpr int Q_BYTES = TM * D * 2, KV_BYTES = KT * D * 2;
-    static constexpr int NB = (232448 - 3584 - NT * Q_BYTES) / KV_BYTES > 6 ? 6 : (232448 - 3584 - NT * Q_BYTES) / KV_BYTES;
+    static constexpr int KS = D <= 128 ? 128 : 64, NS = 2 / NT;  // keys of an S buffer, buffers of a tile
+    static constexpr int Q_BYTES = TM * D * 2, KV_BYTES = KS * D * 2;
+    static constexpr int NB = (232448 - 1792 - NT * Q_BYTES) / KV_BYTES > 6 ? 6 : (232448 - 1792 - NT * Q_BYTES) / KV_BYTES;
     static constexpr int OFF_KV = NT * Q_BYTES, OFF_BAR = OFF_KV + NB * KV_BYTES;
-    static constexpr int OFF_X = OFF_BAR + 256;  // maxima and sums that the two threads of a row exchange
-    static constexpr int OFF_SEG = OFF_X + 2 * 2 * TM * 4;
-    static constexpr int SMEM = OFF_SEG + 256 + 1024;
-    static constexpr int S_COL = 0, O_COL = 2 * KT;  // S buffers, then O
+    static constexpr int OFF_SEG = OFF_BAR + 512;
+    static constexpr int SMEM = OFF_SEG + 256 + 1024;  // slots of 64 bytes
+    static constexpr int S_COL = 0, O_COL = 256;  // S buffers, then O
+    // scores run NS buffers ahead, so the fills from a P's values to their keys are live at once
+    static_assert(2 * NS <= NB, "ring");
     static constexpr int PART = TM * (D + 2);        // floats of a tile's partial rows
 };
 
@@ -107,30 +114,39 @@ __device__ __forceinline__ void tma_3d(void *dst, const CUtensorMap *map, int c0
 }
 
 // Shared-memory descriptors, SWIZZLE_128B, 8-row groups 1024 B apart.  The value
-// tile is read along its rows' values (MN-major): its 64-value column blocks are
-// KT * 128 B apart.
+// fill is read along its rows' values (MN-major): its 64-value column blocks are
+// KS * 128 B apart.
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(KT * 128 / 16) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+template <int KS> __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | ((uint64_t)(KS * 128 / 16) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 template <bool F16> __device__ __forceinline__ constexpr uint32_t idesc(int n, bool b_mn) {
     const uint32_t fmt = F16 ? 0u : 1u;
     return (1u << 4) | (fmt << 7) | (fmt << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(TM >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc)
+// One lane issues, by predicate and not by a branch: the warp stays converged, so
+// descriptors and addresses are computed once in uniform registers, where these
+// instructions take them (under a branch each operand had to be moved there, and
+// an 8-step product took 90 clocks a step beside the softmax warps instead of 64).
+__device__ __forceinline__ void mma_ss(bool lead, uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+                 " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc),
+                 "r"((uint32_t)lead)
                  : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc)
+__device__ __forceinline__ void mma_ts(bool lead, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n"
+                 " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc),
+                 "r"((uint32_t)lead)
                  : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void commit(bool lead, uint64_t *bar) {
+    asm volatile("{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n"
+                 " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+                 "r"((uint32_t)lead)
+                 : "memory");
 }
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -153,20 +169,42 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
 #define KQ_LIST16 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}"
 
-// 32 (16) columns of this warp's 32 lanes; the registers hold them after tmem_wait_ld
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 " KQ_LIST32 ", [%32];" : KQ_R32(r, 0) : "r"(addr));
+// 16 lanes of tensor memory in the layout of a warp's matrix fragments: thread 4g + q
+// has of each 8 f32 columns the columns 2q, 2q + 1 of lanes g (r[4i], r[4i + 1]) and
+// g + 8 (r[4i + 2], r[4i + 3]); of each 4 columns of packed pairs the column q of the
+// two lanes.  A row's values so stay in one warp, in four threads.  Registers hold
+// what was read after tmem_wait_ld.
+__device__ __forceinline__ void tmem_ld_c32(uint32_t addr, uint32_t *r) {  // 32 columns
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 " KQ_LIST16 ", [%16];" : KQ_R16(r) : "r"(addr));
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t *r) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 " KQ_LIST16 ", [%16];" : KQ_R16(r) : "r"(addr));
+__device__ __forceinline__ void tmem_ld_c64(uint32_t addr, uint32_t *r) {  // 64 columns
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 " KQ_LIST32 ", [%32];" : KQ_R32(r, 0) : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t *r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], " KQ_LIST16 ";" ::KQ_U16(r), "r"(addr) : "memory");
+__device__ __forceinline__ void tmem_st_c32(uint32_t addr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], " KQ_LIST16 ";" ::KQ_U16(r), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_st_pairs32(uint32_t addr, const uint32_t *r) {  // 32 columns of packed pairs
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], " KQ_LIST16 ";" ::KQ_U16(r), "r"(addr) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // orders every use of r behind the wait before it
 __device__ __forceinline__ void pin(uint32_t &r) { asm volatile("" : "+r"(r)); }
+
+// w[g] of thread q of a quad <-> w[q] of thread g
+__device__ __forceinline__ void quad_transpose(uint32_t w[4], int lane) {
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            if (g & o) continue;
+            const uint32_t give = up ? w[g] : w[g | o], got = __shfl_xor_sync(0xffffffffu, give, o);
+            if (up) w[g] = got;
+            else w[g | o] = got;
+        }
+    }
+}
 
 // Arithmetic on pairs of f32 in a 64-bit register.
 __device__ __forceinline__ uint64_t pack2u(uint32_t x, uint32_t y) {
@@ -195,6 +233,13 @@ __device__ __forceinline__ float max3f(uint32_t x, uint32_t y, uint32_t z) {
     float v;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(__uint_as_float(x)), "f"(__uint_as_float(y)), "f"(__uint_as_float(z)));
     return v;
+}
+
+// The larger of m and a row's values in a fragment of 64 columns.
+__device__ __forceinline__ float largest(float m, const uint32_t *x, int row) {
+#pragma unroll
+    for (int k = 0; k < 32; k += 4) m = max3f(__float_as_uint(m), x[k + 2 * row], x[k + 2 * row + 1]);
+    return m;
 }
 
 // 2^x of a pair.  The SFU gives 16 results a clock and SM, half of what the
@@ -227,15 +272,15 @@ __device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
 // Capped scores in units of log2.  While |x * in| <= 1 for all of a warp's (a score
 // within the cap: as good as always) the tanh is an odd polynomial, whose largest
 // relative error on that interval is smallest (6.7e-7), and leaves the SFU alone.
-__device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
+template <int N> __device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) m = max3f(__float_as_uint(m), x[i] & 0x7fffffffu, x[i + 1] & 0x7fffffffu);
+    for (int i = 0; i < N; i += 2) m = max3f(__float_as_uint(m), x[i] & 0x7fffffffu, x[i + 1] & 0x7fffffffu);
     if (__all_sync(0xffffffffu, m * in <= 1.0f)) {
         const float c[6] = {0.9999994039535522f, -0.3332904279232025f, 0.13281433284282684f,
                             -0.051605675369501114f, 0.016743114218115807f, -0.003067060373723507f};
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
+        for (int i = 0; i < N; i += 2) {
             const uint64_t u = mul2(pack2u(x[i], x[i + 1]), pack2f(in, in)), v = mul2(u, u);
             uint64_t y = fma2(v, pack2f(c[5], c[5]), pack2f(c[4], c[4]));
 #pragma unroll
@@ -247,28 +292,18 @@ __device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), in, out));
+        for (int i = 0; i < N; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), in, out));
     }
 }
 
-// Barrier of a warp pair (64 threads) that gives the OR of their predicates.
-__device__ __forceinline__ bool bar_or(int id, bool v) {
-    uint32_t r;
-    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 p, %2, 0;\n barrier.cta.red.or.pred q, %1, 64, p;\n selp.u32 %0, 1, 0, q;\n}\n"
-                 : "=r"(r)
-                 : "r"(id), "r"((uint32_t)v)
-                 : "memory");
-    return r != 0;
-}
-
 // One block's share of a pair of tiles.
-struct Seg {
+struct Seg {  // 64 bytes
     int q0, n, len;        // the request
     int b, h, tok0;        // first token of the pair
     int lo, hi;            // keys its rows see
     int lo_tile, tiles;    // key tiles of the pair
     int k0, k1;            // this block's share of them
-    int c[2];              // key tiles of each tile of rows in the share
+    int c[2];              // S buffers of each tile of rows in the share
     int first, last;       // blocks that share the pair
 };
 
@@ -340,14 +375,16 @@ template <int D> struct Walk {
             const int t0 = s.tok0 + i * p.tile_tok, t1 = min(rq.n, t0 + p.tile_tok);
             int l, e;
             key_range(p.a, rq, t0, t1, l, e);
-            const int own = i < NT && t0 < rq.n && e > l ? (e + KT - 1) / KT - s.lo_tile : 0;
-            s.c[i] = max(0, min(min(s.k1, s.tiles), own) - s.k0);
+            constexpr int KS = TL<D>::KS;
+            const int own = i < NT && t0 < rq.n && e > l ? (e + KS - 1) / KS - s.lo_tile * (KT / KS) : 0;
+            s.c[i] = max(0, min(min(s.k1, s.tiles) * (KT / KS), own) - s.k0 * (KT / KS));
         }
         return true;
     }
 };
 
 // Reader's side of the slots: a warp takes the next share and gives it back.
+constexpr int SLOTS = 4;
 struct Shares {
     uint64_t *full, *empty;
     const Seg *slots;
@@ -355,19 +392,19 @@ struct Shares {
     int *err;
     uint32_t i;
     __device__ __forceinline__ const Seg *take() {  // null: no more
-        if (!wait_b(&full[i & 1], (i >> 1) & 1, abort, err, 39)) return nullptr;
-        const Seg *s = slots + (i & 1);
+        if (!wait_b(&full[i % SLOTS], (i / SLOTS) & 1, abort, err, 39)) return nullptr;
+        const Seg *s = slots + i % SLOTS;
         return s->n > 0 ? s : nullptr;
     }
     __device__ __forceinline__ void give(int lane) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[i & 1]);
+        if (lane == 0) mbar_arrive(&empty[i % SLOTS]);
         i++;
     }
 };
 
-// Partial rows of a tile that block `blk` cut: its last pair when it begins the
-// pair, else its first.
+// Partial rows of a tile that block `blk` cut -- its last pair when it begins the
+// pair, else its first: m [128], l [128], unnormalised f32 rows [128][D].
 template <int D> __device__ __forceinline__ float *part_of(float *base, int blk, bool begins, int t) {
     return base + SPLIT_FLOATS + (int64_t)((blk * 2 + (begins ? 1 : 0)) * TL<D>::NT + t) * TL<D>::PART;
 }
@@ -377,23 +414,25 @@ __global__ void __launch_bounds__(THREADS, 1)
     tiles_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                  const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ TileArgs p) {
     using L = TL<D>;
-    constexpr int NT = L::NT, NB = L::NB;
+    constexpr int NT = L::NT, NB = L::NB, KS = L::KS, NS = L::NS;
     const AttnArgs &a = p.a;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *kv_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *kv_empty = kv_full + NB;
-    uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *s_full = q_empty + 1, *p_full = s_full + 2, *o_full = p_full + 2;
-    uint64_t *seg_full = o_full + 2, *seg_empty = seg_full + 2;
+    uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *v_fix = q_empty + 1;
+    uint64_t *s_full = v_fix + 1, *p_full = s_full + 2;  // [buffer]
+    uint64_t *o_full = p_full + 2, *drained = o_full + 2;  // [tile]
+    uint64_t *seg_full = drained + 2, *seg_empty = seg_full + SLOTS;
     Seg *segs = reinterpret_cast<Seg *>(smem + L::OFF_SEG);
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + 2);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + SLOTS);
     volatile int *s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;  // warp: known uniform
 
     if (tid == 0) {
-        for (int i = 0; i < NB; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], 1);
-        mbar_init(q_full, 1), mbar_init(q_empty, 1);
-        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&o_full[i], 1);
-        for (int i = 0; i < 2; i++) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 3 + 8 * NT);
+        for (int i = 0; i < NB; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], NT);
+        mbar_init(q_full, 1), mbar_init(q_empty, NT), mbar_init(v_fix, 1);
+        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&o_full[i], 1), mbar_init(&drained[i], 1);
+        for (int i = 0; i < SLOTS; i++) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 1 + 9 * NT);
         *s_abort = 0;
         fence_mbar_init();
     }
@@ -439,15 +478,31 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     Shares shares{seg_full, seg_empty, segs, s_abort, a.err, 0};
     if (warp >= SOFT_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(OTHER_REGS));
         if (warp == K_WARP || warp == V_WARP) {
             // box r of a tile: keys [r << shift, (r + 1) << shift) of one page, for each
             // 64 values of the head; the pages of the next tile are looked up while
             // this one waits for its place in the ring
-            const int kv = warp == V_WARP, shift = p.box_shift, nrow = KT >> shift;
+            const int kv = warp == V_WARP, shift = p.box_shift, nrow = KS >> shift;
             const CUtensorMap *map = kv ? &tm_v : &tm_k;
             bool bad_page = false;
-            uint32_t fill = kv, items = 0;  // keys take the even fills of the ring, values the odd ones
-            for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
+            uint32_t fill = kv, items = 0, fixes = 0;  // keys take the even fills of the ring, values the odd ones
+            Walk<D> walk(p, whole, ub, kv ? ub : ue, run * per, run_before);
+            auto hand_out = [&]() -> const Seg * {  // the next share, for everyone
+                Seg next;
+                if (!walk.next(next, total, grid)) next.n = 0;
+                if (!wait_b(&seg_empty[shares.i % SLOTS], ((shares.i / SLOTS) & 1) ^ 1, s_abort, a.err, 40)) return nullptr;
+                Seg *s = segs + shares.i % SLOTS;
+                if (lane == 0) {
+                    *s = next;
+                    mbar_arrive(&seg_full[shares.i % SLOTS]);
+                }
+                __syncwarp();
+                shares.i++;
+                return next.n > 0 ? s : nullptr;
+            };
+            // (warp 8 gives nothing back: its slot is only written again by itself)
+            for (const Seg *sp; (sp = kv ? shares.take() : hand_out()) != nullptr; kv ? shares.give(lane) : (void)0) {
                 const int n = max(sp->c[0], sp->c[1]), h = sp->h, lo = sp->lo, hi = sp->hi, key00 = (sp->lo_tile + sp->k0) * KT;
                 if (n == 0) continue;
                 const int32_t *bt = a.table + (int64_t)sp->b * a.table_stride;
@@ -455,7 +510,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 auto look_up = [&](int j) {
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
-                        const int r = lane + 32 * q, key = key00 + j * KT + (r << shift);
+                        const int r = lane + 32 * q, key = key00 + j * KS + (r << shift);
                         page[q] = a.n_pages, off[q] = 0;  // out of bounds: zeros
                         if (r < nrow && key < hi && key + (1 << shift) > lo) {
                             const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
@@ -484,7 +539,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int slot = fill % NB;
                     uint8_t *dst = smem + L::OFF_KV + slot * L::KV_BYTES;
                     const bool ok = wait_b(&kv_empty[slot], ((fill / NB) & 1) ^ 1, s_abort, a.err, 32);
-                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], L::KV_BYTES);
+                    // a page's rows that no row sees may hold anything, and 0 * NaN is NaN:
+                    // such values are cleared here before the tensor core sees them
+                    const int tile0 = key00 + j * KS;
+                    const bool fix = kv && (tile0 < lo || tile0 + KS > hi);
+                    uint64_t *full = fix ? v_fix : &kv_full[slot];
+                    if (lane == 0) mbar_arrive_expect_tx(full, L::KV_BYTES);
                     __syncwarp();
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
@@ -492,7 +552,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (r < nrow && ok)
 #pragma unroll
                             for (int d = 0; d < D / 64; d++)
-                                tma_4d(dst + d * KT * 128 + (r << shift) * 128, map, d * 64, off[q], h, page[q], &kv_full[slot]);
+                                tma_4d(dst + d * KS * 128 + (r << shift) * 128, map, d * 64, off[q], h, page[q], full);
+                    }
+                    if (fix) {
+                        wait_b(v_fix, fixes++ & 1, s_abort, a.err, 34);
+                        for (int i = lane; i < KS * 8; i += 32) {
+                            const int key = tile0 + (i >> 3);
+                            if (key >= lo && key < hi) continue;
+#pragma unroll
+                            for (int d = 0; d < D / 64; d++)
+                                *reinterpret_cast<uint4 *>(dst + d * KS * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async_shared();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&kv_full[slot]);
                     }
                     if (j + 1 < n) look_up(j + 1);
                 }
@@ -501,300 +574,280 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (*s_abort)  // nothing consumes what is still in flight: let it land before the block ends
                 for (uint32_t f = fill >= 2 * NB + kv ? fill - 2 * NB : kv; f < fill; f += 2)
                     mbar_wait(&kv_full[f % NB], (f / NB) & 1, 1u << 20);
-        } else if (warp == MMA_WARP) {
-            constexpr uint32_t id_s = idesc<F16>(KT, false), id_o = idesc<F16>(D, true);
-            uint32_t takes = 0, items = 0, np[2] = {0, 0}, ns = 0;
+        } else if (warp < MMA_WARP + NT) {
+            constexpr uint32_t id_s = idesc<F16>(KS, false), id_o = idesc<F16>(D, true);
+            const int t = warp - MMA_WARP;
+            const uint64_t dq = desc_k(smem_u32(smem + t * L::Q_BYTES)), dk0 = desc_k(smem_u32(smem + L::OFF_KV));
+            const uint64_t dv0 = desc_mn<KS>(smem_u32(smem + L::OFF_KV));
+            const uint32_t d_s = tmem + L::S_COL + t * KS, d_o = tmem + L::O_COL + t * D;
+            const bool lead = lane == 0;
+            uint32_t items = 0, pp = 0;               // pp: a parity bit for each buffer's p_full
+            uint32_t kf = 0, kp = 0, vf = 1, vp = 0;  // the ring's next fill of keys and of values, and its parity
+            auto step = [](uint32_t &f, uint32_t &par) {
+                f += 2;
+                if (f >= NB) f -= NB, par ^= 1;
+            };
             for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
-                const Seg s = *sp;
-                const int n = max(s.c[0], s.c[1]);
+                const int c = __shfl_sync(0xffffffffu, sp->c[t], 0), n = __shfl_sync(0xffffffffu, max(sp->c[0], sp->c[1]), 0);
                 if (n == 0) continue;
-                wait_b(q_full, items & 1, s_abort, a.err, 33);
+                bool ok = wait_b(q_full, items & 1, s_abort, a.err, 33);
                 items++;
-                auto qk = [&](int t, int buf, uint32_t take) {  // S[buf] = Q[t] K^T
-                    if (lane == 0 && !*s_abort) {
-                        const uint32_t sq = smem_u32(smem + t * L::Q_BYTES), sk = smem_u32(smem + L::OFF_KV + (take % NB) * L::KV_BYTES);
+                // Scores S = Q K^T run NS steps ahead of the product that frees their buffer.
+                // The commit behind them tells the softmax that they are there, and that the
+                // products before them are done.  The last product has a barrier of its own:
+                // the next share's first scores need nothing from the softmax, and could run
+                // past a phase that a slow warp still waits for.
+                // A tile that has no use for a fill waits for it all the same before giving it
+                // back, or it could give it back twice while the other tile still reads it.
+                auto scores = [&](int i) {
+                    ok = wait_b(&kv_full[kf], kp, s_abort, a.err, 34) && ok;
+                    if (i < c) {
+                        const uint64_t dk = dk0 + kf * (L::KV_BYTES / 16);
 #pragma unroll
                         for (int kk = 0; kk < D / 16; kk++)
-                            mma_ss(tmem + L::S_COL + buf * KT, desc_k(sq + (kk >> 2) * TM * 128 + (kk & 3) * 32),
-                                   desc_k(sk + (kk >> 2) * KT * 128 + (kk & 3) * 32), id_s, kk ? 1u : 0u);
-                    }
-                    if (lane == 0) commit(&s_full[buf]);
-                };
-                auto pv = [&](int t, int buf, uint32_t take, bool acc) {  // O[t] += P[buf] V
-                    if (lane == 0 && !*s_abort) {
-                        const uint32_t sv = smem_u32(smem + L::OFF_KV + (take % NB) * L::KV_BYTES);
-#pragma unroll
-                        for (int kk = 0; kk < KT / 16; kk++)
-                            mma_ts(tmem + L::O_COL + t * D, tmem + L::S_COL + buf * KT + (kk >> 1) * 32 + (kk & 1) * 8, desc_mn(sv + kk * 2048), id_o,
-                                   acc || kk ? 1u : 0u);
-                    }
-                    if (lane == 0) commit(&o_full[t]);
-                };
-                auto full = [&](uint32_t take) {
-                    wait_b(&kv_full[take % NB], (take / NB) & 1, s_abort, a.err, 34);
-                    tc_after();
-                };
-                auto release = [&](uint32_t take) {
-                    if (lane == 0) commit(&kv_empty[take % NB]);
-                };
-                auto values = [&](uint32_t take, int j) {  // a page's rows that no row sees may hold anything: 0 * NaN
-                    full(take);
-                    const int tile0 = (s.lo_tile + s.k0 + j) * KT;
-                    if (tile0 < s.lo || tile0 + KT > s.hi) {
-                        uint8_t *sv = smem + L::OFF_KV + (take % NB) * L::KV_BYTES;
-                        const int from = min(max(s.hi - tile0, 0), KT), to = min(max(s.lo - tile0, 0), KT);
-                        for (int i = lane; i < KT * 8; i += 32) {
-                            const int r = i >> 3;
-                            if (r >= to && r < from) continue;
-#pragma unroll
-                            for (int d = 0; d < D / 64; d++)
-                                *reinterpret_cast<uint4 *>(sv + d * KT * 128 + r * 128 + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_async_shared();
-                        __syncwarp();
+                            mma_ss(lead && ok, d_s + (i % NS) * KS, dq + (kk >> 2) * (TM * 8) + (kk & 3) * 2,
+                                   dk + (kk >> 2) * (KS * 8) + (kk & 3) * 2, id_s, kk ? 1u : 0u);
                     }
                 };
-                if constexpr (NT == 2) {
-                    full(takes);
-#pragma unroll
-                    for (int t = 0; t < 2; t++)
-                        if (s.c[t] > 0) qk(t, t, takes);
-                    release(takes);
-                    if (n == 1 && lane == 0) commit(q_empty);
-                    for (int j = 0; j < n; j++) {
-                        const uint32_t tv = takes + 2 * j + 1, tk = tv + 1;
-                        values(tv, j);
-#pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            if (j < s.c[t]) {
-                                wait_b(&p_full[t], np[t]++ & 1, s_abort, a.err, 35);
-                                tc_after();
-                                pv(t, t, tv, j > 0);
-                            }
-                            if (t == 0 && j + 1 < n) full(tk);
-                            if (j + 1 < s.c[t]) qk(t, t, tk);
-                        }
-                        release(tv);
-                        if (j + 1 < n) release(tk);
-                        if (j + 2 == n && lane == 0) commit(q_empty);
-                    }
-                } else {
-                    full(takes);
-                    qk(0, ns & 1, takes);
-                    release(takes);
-                    if (n == 1 && lane == 0) commit(q_empty);
-                    for (int j = 0; j < n; j++, ns++) {
-                        const uint32_t tv = takes + 2 * j + 1, tk = tv + 1;
-                        values(tv, j);
-                        if (j + 1 < n) {
-                            full(tk);
-                            qk(0, (ns + 1) & 1, tk);
-                            release(tk);
-                            if (j + 2 == n && lane == 0) commit(q_empty);
-                        }
-                        wait_b(&p_full[ns & 1], np[ns & 1]++ & 1, s_abort, a.err, 35);
+                auto behind = [&](int i) {
+                    commit(lead, &kv_empty[kf]);
+                    step(kf, kp);
+                    if (i == n - 1) commit(lead, q_empty);
+                };
+                for (int i = 0; i < NS && i < n; i++) {
+                    scores(i);
+                    if (i < c) commit(lead, &s_full[t * NS + i]);
+                    behind(i);
+                }
+                for (int i = 0; i < n; i++) {
+                    const int b = i % NS;
+                    ok = wait_b(&kv_full[vf], vp, s_abort, a.err, 34) && ok;
+                    if (i < c) {  // O += P V
+                        const uint64_t dv = dv0 + vf * (L::KV_BYTES / 16);
+                        ok = wait_b(&p_full[t * NS + b], (pp >> b) & 1, s_abort, a.err, 35) && ok;
+                        pp ^= 1u << b;
                         tc_after();
-                        pv(0, ns & 1, tv, j > 0);
-                        release(tv);
+#pragma unroll
+                        for (int kk = 0; kk < KS / 16; kk++)
+                            mma_ts(lead && ok, d_o, d_s + b * KS + kk * 8, dv + kk * 128, id_o, i > 0 || kk ? 1u : 0u);
                     }
+                    if (i < c && (NS > 1 || i == c - 1)) commit(lead, &o_full[t]);
+                    if (i + NS < n) {
+                        scores(i + NS);
+                        if (i + NS < c) commit(lead, &s_full[t * NS + b]);
+                        behind(i + NS);
+                    }
+                    commit(lead, &kv_empty[vf]);
+                    step(vf, vp);
                 }
-                takes += 2 * n;
             }
-        } else if (warp == WALK_WARP) {
-            Walk<D> walk(p, whole, ub, ue, run * per, run_before);
-            Seg s;
-            for (uint32_t i = 0;; i++) {
-                const bool more = walk.next(s, total, grid);
-                if (!more) s.n = 0;
-                if (!wait_b(&seg_empty[i & 1], ((i >> 1) & 1) ^ 1, s_abort, a.err, 40)) break;
-                if (lane == 0) {
-                    segs[i & 1] = s;
-                    mbar_arrive(&seg_full[i & 1]);
-                }
-                if (!more) break;
-            }
+            // no arrival is on its way to shared memory when the block ends
+            commit(lead, &drained[t]);
+            wait_b(&drained[t], 0, s_abort, a.err, 37);
         }
-    } else if (NT == 2 || warp < 8) {
-        // softmax: thread (row, half) has 64 of the 128 keys of a row of tile t; the
-        // two threads of a row sit in warps w and w + 4, joined by a barrier of 64
-        const int t = warp >> 3, half = (warp >> 2) & 1, row = tid & 127, pair_bar = 1 + t * 4 + (warp & 3);
-        float *xch = reinterpret_cast<float *>(smem + L::OFF_X) + t * 2 * TM;
-        const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane 32 * (warp % 4)
-        const uint32_t o_addr = tmem + lanes + L::O_COL + (NT == 2 ? t : 0) * D + half * (D / 2);
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SOFT_REGS));
+        // softmax of 16 rows of tile t: this thread has 2 of each 8 keys of rows[0], rows[1]
+        const int t = warp >> 3, q2 = (lane & 3) * 2;
+        const int row0 = (warp & 3) * 32 + (warp >> 2 & 1) * 16 + (lane >> 2);  // and row0 + 8
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32 + (warp >> 2 & 1) * 16) << 16;
+        const uint32_t o_addr = tmem + lanes + L::O_COL + t * D;
         const float sl2 = CAP ? 1.0f : a.scale * LOG2E;
         const float cap_in = CAP ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
-        const float slack = 8.0f / sl2;  // the reference lags the maximum by up to 2^8
         const uint64_t sl2_2 = pack2f(sl2, sl2);
-        uint32_t nsf = 0, no = 0;        // S tiles and P V products of this tile so far
-        for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
+        uint32_t sp_bits = 0;            // a parity bit for each of the tile's s_full
+        uint32_t no = 0;                 // products that o_full has told of (NS 1: of shares)
+        auto wait_o = [&] {
+            wait_b(&o_full[t], no++ & 1, s_abort, a.err, 38);
+            __syncwarp();
+            tc_after();
+        };
+        for (const Seg *sp; t < NT && (sp = shares.take()) != nullptr; shares.give(lane)) {
             const volatile Seg &s = *sp;
-            const int tok = s.tok0 + t * p.tile_tok + row / a.G;
-            const int live_tok = min(s.n, s.tok0 + (t + 1) * p.tile_tok);
-            const bool live = row < p.tile_tok * a.G && tok < live_tok;
-            const int shift = s.len - s.n + 1, mtok = min(tok, live_tok - 1);
-            const int lim = a.causal ? shift + mtok : s.len, low = a.window ? lim - a.window : 0;
+            const int tok0 = s.tok0 + t * p.tile_tok, live_tok = min(s.n, tok0 + p.tile_tok);
+            const int shift = s.len - s.n + 1;
+            bool live[2];
+            int lim[2], low[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int row = row0 + 8 * r, tok = tok0 + row / a.G;
+                live[r] = row < p.tile_tok * a.G && tok < live_tok;
+                lim[r] = a.causal ? shift + min(tok, live_tok - 1) : s.len, low[r] = a.window ? lim[r] - a.window : 0;
+            }
             // keys that every row of the tile sees
-            const int all_hi = a.causal ? shift + s.tok0 + t * p.tile_tok : s.len, all_lo = a.window ? shift + live_tok - 1 - a.window : 0;
-            float ref = -INFINITY, l = 0.f;
+            const int all_hi = a.causal ? shift + tok0 : s.len, all_lo = a.window ? shift + live_tok - 1 - a.window : 0;
+            float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+            const uint32_t o_base = no;
             const int c = s.c[t], first_key = (s.lo_tile + s.k0) * KT;
-            for (int j = 0; j < c; j++) {
-                const int buf = NT == 2 ? t : (int)(nsf & 1), key0 = first_key + j * KT;
-                const uint32_t s_addr = tmem + lanes + L::S_COL + buf * KT;
-                wait_b(&s_full[buf], NT == 2 ? nsf & 1 : (nsf >> 1) & 1, s_abort, a.err, 36);
-                nsf++;
+            for (int i = 0; i < c; i++) {
+                const int key0 = first_key + i * KS;
+                const uint32_t s_addr = tmem + lanes + L::S_COL + (t * NS + i % NS) * KS;
+                wait_b(&s_full[t * NS + i % NS], (sp_bits >> (i % NS)) & 1, s_abort, a.err, 36);
+                sp_bits ^= 1u << (i % NS);
+                __syncwarp();  // tensor memory is read by whole warps
                 tc_after();
-                // S in two chunks of 32 keys: the second stays in registers, the first is read
-                // again for its exponentials (holding both would not leave enough registers)
-                uint32_t x[32];
-                auto load = [&](int chunk, bool again) {
-                    tmem_ld32(s_addr + half * HC + chunk * 32, x);
+                // (a phase is told from the one before the last only by who waits for both)
+                while (NS > 1 && (int)(no - o_base) < i - 1) wait_o();
+                uint32_t x[32], pk[KS / 4];
+                auto load = [&](int g) {  // 64 columns
+                    tmem_ld_c64(s_addr + g, x);
                     tmem_wait_ld();
-                    const int k = key0 + half * HC + chunk * 32;
 #pragma unroll
-                    for (int i = 0; i < 32; i++) pin(x[i]);
-                    if (CAP && again) return;
-                    if (CAP) cap_scores(x, cap_in, cap_out);
-                    if (key0 + KT > all_hi || key0 < all_lo) {
+                    for (int k = 0; k < 32; k++) pin(x[k]);
+                    if (CAP) cap_scores<32>(x, cap_in, cap_out);
+                    if (key0 + KS > all_hi || key0 < all_lo) {
 #pragma unroll
-                        for (int i = 0; i < 32; i++) x[i] = k + i < lim && k + i >= low ? x[i] : 0xff800000u;
-                    }
-                    if (CAP && chunk == 0) {  // what is read again
-                        tmem_st16(s_addr + half * HC, x);
-                        tmem_st16(s_addr + half * HC + 16, x + 16);
-                        tmem_wait_st();
+                        for (int k = 0; k < 32; k++) {
+                            const int key = key0 + g + q2 + k / 4 * 8 + (k & 1), r = k >> 1 & 1;
+                            x[k] = key < lim[r] && key >= low[r] ? x[k] : 0xff800000u;
+                        }
                     }
                 };
-                auto largest = [&] {
-                    float m0 = max3f(x[0], x[1], x[2]), m1 = max3f(x[3], x[4], x[5]);
+                // P, O and l are kept relative to `ref`: the largest score of the first keys
+                // that the row sees.  A softmax needs no more than that as long as nothing
+                // overflows, since P and f32 are floating-point: bf16 bears a sum of 2^60,
+                // f16 one of 2^13 a thread.  So the maximum of later keys is only taken when
+                // the sum of their probabilities (or the exponent of one that exp2_poly
+                // would wrap) asks for it, and then they are taken again.
+                float sum[2];
+                for (bool fresh = i == 0;; fresh = false) {
+                    bool again = fresh;
+                    if (!fresh) {
+                        uint64_t base2[2], l2[2] = {0, 0};
+                        float top = 0.f;
 #pragma unroll
-                    for (int i = 6; i < 30; i += 4) {
-                        m0 = max3f(__float_as_uint(m0), x[i], x[i + 1]);
-                        m1 = max3f(__float_as_uint(m1), x[i + 2], x[i + 3]);
+                        for (int r = 0; r < 2; r++) {
+                            const float base = ref[r] == -INFINITY ? 0.f : -ref[r] * sl2;
+                            base2[r] = pack2f(base, base);
+                        }
+#pragma unroll
+                        for (int g = 0; g < KS; g += 64) {
+                            load(g);
+#pragma unroll
+                            for (int k = 0; k < 16; k++) {
+                                const int r = k & 1;
+                                uint64_t y = fma2(pack2u(x[2 * k], x[2 * k + 1]), sl2_2, base2[r]);
+                                float p0, p1;
+                                if (k % 8 < POLY) {
+                                    unpack2f(y, p0, p1);
+                                    top = max3f(__float_as_uint(top), __float_as_uint(p0), __float_as_uint(p1));
+                                    y = exp2_poly(y);
+                                } else y = exp2_mufu(y);
+                                l2[r] = add2(l2[r], y);
+                                unpack2f(y, p0, p1);
+                                pk[g / 4 + k] = pack_half<F16>(p0, p1);  // rounded to the values' type for the product
+                            }
+                        }
+                        bool high = top > 100.f, none = false;
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            float la, lb;
+                            unpack2f(l2[r], la, lb);
+                            sum[r] = la + lb;
+                            high |= sum[r] > (F16 ? 0x1p13f : 0x1p60f);
+                            none |= live[r] && ref[r] == -INFINITY;
+                        }
+                        again = (high && (live[0] || live[1])) || none;
                     }
-                    return max3f(__float_as_uint(m0), __float_as_uint(m1), __float_as_uint(fmaxf(__uint_as_float(x[30]), __uint_as_float(x[31]))));
-                };
-                load(0, false);
-                float mx = largest();
-                load(1, false);
-                mx = fmaxf(mx, largest());
-                // O and l are kept relative to `ref`, which follows the maximum only when
-                // that has outgrown it by 2^8 (P's type and f32 both hold the excess), so
-                // the two threads of a row mostly need no more than this one vote
-                if (bar_or(pair_bar, j == 0 || mx > ref + slack)) {
-                    xch[half * TM + row] = mx;
-                    named_bar_sync(pair_bar, 64);
-                    mx = fmaxf(mx, xch[(half ^ 1) * TM + row]);
-                    if (j == 0) ref = mx;
-                    else {
-                        const float to = mx > ref + slack ? mx : ref;
-                        const float k = to == ref ? 1.0f : ex2((ref - to) * sl2);  // 0 when nothing was seen before
-                        l *= k;
-                        ref = to;
-                        wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 37);
-                        tc_after();
+                    if (!__any_sync(0xffffffffu, again)) break;
+                    float to[2] = {ref[0], ref[1]};
 #pragma unroll 1
-                        for (int d = 0; d < D / 2; d += 16) {
+                    for (int g = 0; g < KS; g += 64) {
+                        load(g);
+                        to[0] = largest(to[0], x, 0), to[1] = largest(to[1], x, 1);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        to[r] = fmaxf(to[r], __shfl_xor_sync(0xffffffffu, to[r], 1));
+                        to[r] = fmaxf(to[r], __shfl_xor_sync(0xffffffffu, to[r], 2));
+                    }
+                    // (no way on: every row's reference is its maximum -- rows without a key so
+                    // far, or scores that overflow f32)
+                    if (!__any_sync(0xffffffffu, fresh || (live[0] && to[0] > ref[0]) || (live[1] && to[1] > ref[1]))) break;
+                    float k[2];
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        k[r] = to[r] == ref[r] || i == 0 ? 1.0f : ex2((ref[r] - to[r]) * sl2);
+                        l[r] *= k[r];
+                        ref[r] = to[r];
+                    }
+                    if (i > 0) {
+                        while (NS > 1 && (int)(no - o_base) < i) wait_o();  // the last product (NS 1: this S is behind it)
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 32) {
                             uint32_t o[16];
-                            tmem_ld16(o_addr + d, o);
+                            tmem_ld_c32(o_addr + d, o);
                             tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 16; i++) {
-                                pin(o[i]);
-                                o[i] = __float_as_uint(__uint_as_float(o[i]) * k);
+                            for (int e = 0; e < 16; e++) {
+                                pin(o[e]);
+                                o[e] = __float_as_uint(__uint_as_float(o[e]) * k[e >> 1 & 1]);
                             }
-                            tmem_st16(o_addr + d, o);
+                            tmem_st_c32(o_addr + d, o);
                         }
                     }
                 }
-                const float base = ref == -INFINITY ? 0.f : -ref * sl2;
-                const uint64_t base2 = pack2f(base, base);
-                uint64_t l2 = 0;
 #pragma unroll
-                for (int chunk = 1; chunk >= 0; chunk--) {
-                    if (chunk == 0) load(0, true);
-                    uint32_t pk[16];
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        uint64_t y = fma2(pack2u(x[2 * i], x[2 * i + 1]), sl2_2, base2);
-                        y = i % 8 < POLY ? exp2_poly(y) : exp2_mufu(y);
-                        l2 = add2(l2, y);
-                        // rounded to the values' type for the product; the sum stays in f32
-                        float p0, p1;
-                        unpack2f(y, p0, p1);
-                        pk[i] = pack_half<F16>(p0, p1);
-                    }
-                    tmem_st16(s_addr + half * HC + chunk * 32, pk);  // over the scores it came from
-                }
-                float la, lb;
-                unpack2f(l2, la, lb);
-                l += la + lb;
+                for (int g = 0; g < KS / 4; g += 16) tmem_st_pairs32(s_addr + g * 2, pk + g);
+                l[0] += sum[0], l[1] += sum[1];
                 tmem_wait_st();
                 tc_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[buf]);
-                no++;
+                if (lane == 0) mbar_arrive(&p_full[t * NS + i % NS]);
             }
+            if (NS == 1 && c > 0) wait_o();
+            while (NS > 1 && (int)(no - o_base) < c) wait_o();
             // ---- the tile's rows, or this block's part of them
+            if (tok0 >= s.n) continue;
             const int first = s.first, last = s.last;
-            const bool has_tile = s.tok0 + t * p.tile_tok < s.n;
-            if (!has_tile) continue;
-            named_bar_sync(pair_bar, 64);  // the last exchange is read
-            xch[half * TM + row] = l;
-            named_bar_sync(pair_bar, 64);
-            l += xch[(half ^ 1) * TM + row];
-            if (ref == -INFINITY) l = 0.f;  // no key seen (exp2_poly gives a masked one 2^-126)
-            if (c > 0) {
-                wait_b(&o_full[NT == 2 ? t : 0], (no - 1) & 1, s_abort, a.err, 38);
-                tc_after();
-            }
-            const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row % a.G;
-            uint16_t *dst = reinterpret_cast<uint16_t *>(a.out) + orow * D + half * (D / 2);
-            const float ml = ref * sl2;  // log2 units
-            if (first == last) {
-                const float inv = l > 0.f ? 1.0f / l : 0.f;
-#pragma unroll 1
-                for (int d = 0; d < D / 2; d += 32) {
-                    uint32_t o[32];
-                    if (c > 0) {
-                        tmem_ld32(o_addr + d, o);
-                        tmem_wait_ld();
-                    }
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        pin(o[i]);
-                        if (c == 0) o[i] = 0u;
-                    }
-                    if (live)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            uint4 w;
-                            w.x = pack_half<F16>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                            w.y = pack_half<F16>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                            w.z = pack_half<F16>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                            w.w = pack_half<F16>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-                            *reinterpret_cast<uint4 *>(dst + d + i) = w;
-                        }
-                }
-                if (live && half == 0 && a.lse) a.lse[orow] = l > 0.f ? ml * LN2 + logf(l) : -INFINITY;
-                continue;
-            }
-            // partial rows: m, l [128], then float4 [D / 4][128] (a warp's rows side by side)
+            const bool split = first != last;
+            float inv[2];
+            int64_t orow[2];
             float *part = part_of<D>(a.part, blockIdx.x, s.k0 == 0, t);
-            if (half == 0) part[row] = l > 0.f ? ml : -INFINITY, part[TM + row] = l;
-            if (tid == 0 && s.k0 == 0) splits[blockIdx.x] = Split{last, s.q0, s.n, s.tok0, s.h};
-            if (c > 0) {
+            if (split && tid == 0 && s.k0 == 0) splits[blockIdx.x] = Split{last, s.q0, s.n, s.tok0, s.h};
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                const int row = row0 + 8 * r;
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                if (ref[r] == -INFINITY) l[r] = 0.f;  // no key seen: exp2_poly gave 2^-126
+                inv[r] = l[r] > 0.f ? 1.0f / l[r] : 0.f;
+                orow[r] = (int64_t)(s.q0 + tok0 + row / a.G) * a.Hq + s.h * a.G + row % a.G;
+                const float ml = ref[r] * sl2;  // log2 units
+                if (q2 == 0) {
+                    if (split) part[row] = l[r] > 0.f ? ml : -INFINITY, part[TM + row] = l[r];
+                    else if (live[r] && a.lse) a.lse[orow[r]] = l[r] > 0.f ? ml * LN2 + logf(l[r]) : -INFINITY;
+                }
+            }
+            if (split && c == 0) continue;
 #pragma unroll 1
-                for (int d = 0; d < D / 2; d += 32) {
-                    uint32_t o[32];
-                    tmem_ld32(o_addr + d, o);
+            for (int d = 0; d < D; d += 32) {
+                uint32_t o[16];
+                __syncwarp();
+                if (c > 0) {
+                    tmem_ld_c32(o_addr + d, o);
                     tmem_wait_ld();
+                }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) pin(o[i]);
-                    if (live)
+                for (int e = 0; e < 16; e++) {
+                    pin(o[e]);
+                    if (c == 0) o[e] = 0u;
+                }
+                if (split) {  // f32 rows behind m and l
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4 *>(part + 2 * TM + ((half * (D / 2) + d + i) / 4 * TM + row) * 4) =
-                                make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    for (int e = 0; e < 16; e += 2)
+                        if (live[e >> 1 & 1])
+                            *reinterpret_cast<uint2 *>(part + 2 * TM + (row0 + (e >> 1 & 1) * 8) * D + d + e / 4 * 8 + q2) = make_uint2(o[e], o[e + 1]);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int g = 0; g < 4; g++)
+                            w[g] = pack_half<F16>(__uint_as_float(o[g * 4 + r * 2]) * inv[r], __uint_as_float(o[g * 4 + r * 2 + 1]) * inv[r]);
+                        quad_transpose(w, lane);  // the quad's thread q: the 8 columns of group q
+                        if (live[r]) *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.out) + orow[r] * D + d + q2 * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
                 }
             }
         }
@@ -805,42 +858,42 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// Joins the pair that block blockIdx.x of the tiles began and others ended: 32 of
-// its rows (blockIdx.y), a lane a row, each warp every eighth float4 of them.
-constexpr int JOIN_ROWS = 32, JOIN_WARPS = 8;
-template <bool F16, int D> __global__ void __launch_bounds__(JOIN_WARPS * 32) join_kernel(const __grid_constant__ TileArgs p) {
+// Joins the pair that block blockIdx.x of the tiles began and others ended: 16 of
+// its rows (blockIdx.y), 16 threads a row.
+constexpr int JOIN_ROWS = 16, JOIN_T = 256;
+template <bool F16, int D> __global__ void __launch_bounds__(JOIN_T) join_kernel(const __grid_constant__ TileArgs p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const AttnArgs &a = p.a;
-    const int first = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int first = blockIdx.x, sub = threadIdx.x & 15;
     const Split s = reinterpret_cast<const Split *>(a.part)[first];
     if (s.last == first) return;
-    const int t = blockIdx.y * JOIN_ROWS / TM, row = blockIdx.y * JOIN_ROWS % TM + lane;
+    const int t = blockIdx.y * JOIN_ROWS / TM, row = blockIdx.y * JOIN_ROWS % TM + (threadIdx.x >> 4);
     const int tok = s.tok0 + t * p.tile_tok + row / a.G;
     if (row >= p.tile_tok * a.G || tok >= min(s.n, s.tok0 + (t + 1) * p.tile_tok)) return;
     float m = -INFINITY, l = 0.f;
 #pragma unroll 4
     for (int b = first; b <= s.last; b++) m = fmaxf(m, part_of<D>(a.part, b, b == first, t)[row]);
-    float4 acc[D / 4 / JOIN_WARPS];
+    float4 acc[D / 64];
 #pragma unroll
-    for (int i = 0; i < D / 4 / JOIN_WARPS; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+    for (int i = 0; i < D / 64; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int b = first; b <= s.last; b++) {
         const float *q = part_of<D>(a.part, b, b == first, t);
         const float mb = q[row], w = mb == -INFINITY ? 0.f : ex2(mb - m);
         l += w * q[TM + row];
 #pragma unroll
-        for (int i = 0; i < D / 4 / JOIN_WARPS; i++) {
-            const float4 v = reinterpret_cast<const float4 *>(q + 2 * TM)[(warp + i * JOIN_WARPS) * TM + row];
+        for (int i = 0; i < D / 64; i++) {
+            const float4 v = reinterpret_cast<const float4 *>(q + 2 * TM + row * D)[sub + i * 16];
             if (w != 0.f) acc[i].x += w * v.x, acc[i].y += w * v.y, acc[i].z += w * v.z, acc[i].w += w * v.w;
         }
     }
     const float inv = l > 0.f ? 1.0f / l : 0.f;
     const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row % a.G;
 #pragma unroll
-    for (int i = 0; i < D / 4 / JOIN_WARPS; i++)
-        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + (warp + i * JOIN_WARPS) * 4) =
+    for (int i = 0; i < D / 64; i++)
+        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + (sub + i * 16) * 4) =
             make_uint2(pack_half<F16>(acc[i].x * inv, acc[i].y * inv), pack_half<F16>(acc[i].z * inv, acc[i].w * inv));
-    if (warp == 0 && a.lse) a.lse[orow] = l > 0.f ? m * LN2 + logf(l) : -INFINITY;
+    if (sub == 0 && a.lse) a.lse[orow] = l > 0.f ? m * LN2 + logf(l) : -INFINITY;
 }
 
 bool encode(CUtensorMap *m, bool f16, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
@@ -854,8 +907,8 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     using L = TL<D>;
     TileArgs p;
     p.a = a;
-    int shift = 0;  // the largest power of two that divides both a page and a tile
-    while ((1 << shift) < KT && a.page % (2 << shift) == 0) shift++;
+    int shift = 0;  // the largest power of two that divides both a page and a fill
+    while ((1 << shift) < L::KS && a.page % (2 << shift) == 0) shift++;
     p.box_shift = shift;
     p.tile_tok = TM / a.G;
     p.q_tx = (uint32_t)(p.tile_tok * a.G * D * 2);
@@ -879,7 +932,7 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(num_sms(), L::NT * TM / JOIN_ROWS);
-    cfg.blockDim = dim3(JOIN_WARPS * 32);
+    cfg.blockDim = dim3(JOIN_T);
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
