@@ -247,7 +247,7 @@ __device__ __forceinline__ float largest(float m, const uint32_t *x, int row) {
 // x = n + f with |f| <= 1/2 (n by adding 1.5 * 2^23), 2^f by the polynomial of
 // degree 4 whose largest relative error on that interval is smallest (2.7e-6,
 // fitted by exchange of the extrema), and n added to the exponent.
-constexpr int POLY = 3;
+constexpr int POLY = 1;
 __device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
     float u, v;
     unpack2f(x, u, v);
@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *kv_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *kv_empty = kv_full + NB;
     uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *v_fix = q_empty + 1;
     uint64_t *s_full = v_fix + 1, *p_full = s_full + 2;  // [buffer]
-    uint64_t *o_full = p_full + 2, *drained = o_full + 2;  // [tile]
-    uint64_t *seg_full = drained + 2, *seg_empty = seg_full + SLOTS;
+    uint64_t *o_full = p_full + 2, *drained = o_full + 2, *turn = drained + 2;  // [tile]
+    uint64_t *seg_full = turn + 2, *seg_empty = seg_full + SLOTS;
     Seg *segs = reinterpret_cast<Seg *>(smem + L::OFF_SEG);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + SLOTS);
     volatile int *s_abort = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (tid == 0) {
         for (int i = 0; i < NB; i++) mbar_init(&kv_full[i], 1), mbar_init(&kv_empty[i], NT);
         mbar_init(q_full, 1), mbar_init(q_empty, NT), mbar_init(v_fix, 1);
-        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&o_full[i], 1), mbar_init(&drained[i], 1);
+        for (int i = 0; i < 2; i++) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 8), mbar_init(&o_full[i], 1), mbar_init(&drained[i], 1), mbar_init(&turn[i], 1);
         for (int i = 0; i < SLOTS; i++) mbar_init(&seg_full[i], 1), mbar_init(&seg_empty[i], 1 + 9 * NT);
         *s_abort = 0;
         fence_mbar_init();
@@ -581,8 +581,20 @@ __global__ void __launch_bounds__(THREADS, 1)
             const uint64_t dv0 = desc_mn<KS>(smem_u32(smem + L::OFF_KV));
             const uint32_t d_s = tmem + L::S_COL + t * KS, d_o = tmem + L::O_COL + t * D;
             const bool lead = lane == 0;
+            bool ok = true;
             uint32_t items = 0, pp = 0;               // pp: a parity bit for each buffer's p_full
             uint32_t kf = 0, kp = 0, vf = 1, vp = 0;  // the ring's next fill of keys and of values, and its parity
+            // The tiles take turns at the tensor core.  Left alone it would mix their steps, both
+            // tiles would finish together, and so would their softmaxes: tensor core and SFU
+            // would work one after the other, not side by side.
+            uint32_t turns = 0;
+            auto my_turn = [&] {
+                if (NT == 2) ok = wait_b(&turn[t], (turns++ & 1) ^ (t == 0), s_abort, a.err, 33) && ok;
+            };
+            auto your_turn = [&] {
+                if (NT == 2 && lead) mbar_arrive(&turn[t ^ 1]);
+                __syncwarp();
+            };
             auto step = [](uint32_t &f, uint32_t &par) {
                 f += 2;
                 if (f >= NB) f -= NB, par ^= 1;
@@ -590,7 +602,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
                 const int c = __shfl_sync(0xffffffffu, sp->c[t], 0), n = __shfl_sync(0xffffffffu, max(sp->c[0], sp->c[1]), 0);
                 if (n == 0) continue;
-                bool ok = wait_b(q_full, items & 1, s_abort, a.err, 33);
+                ok = wait_b(q_full, items & 1, s_abort, a.err, 33) && ok;
                 items++;
                 // Scores S = Q K^T run NS steps ahead of the product that frees their buffer.
                 // The commit behind them tells the softmax that they are there, and that the
@@ -599,8 +611,8 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // past a phase that a slow warp still waits for.
                 // A tile that has no use for a fill waits for it all the same before giving it
                 // back, or it could give it back twice while the other tile still reads it.
+                auto keys = [&] { ok = wait_b(&kv_full[kf], kp, s_abort, a.err, 34) && ok; };
                 auto scores = [&](int i) {
-                    ok = wait_b(&kv_full[kf], kp, s_abort, a.err, 34) && ok;
                     if (i < c) {
                         const uint64_t dk = dk0 + kf * (L::KV_BYTES / 16);
 #pragma unroll
@@ -615,28 +627,36 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (i == n - 1) commit(lead, q_empty);
                 };
                 for (int i = 0; i < NS && i < n; i++) {
+                    keys();
+                    my_turn();
                     scores(i);
                     if (i < c) commit(lead, &s_full[t * NS + i]);
+                    your_turn();
                     behind(i);
                 }
                 for (int i = 0; i < n; i++) {
                     const int b = i % NS;
                     ok = wait_b(&kv_full[vf], vp, s_abort, a.err, 34) && ok;
-                    if (i < c) {  // O += P V
-                        const uint64_t dv = dv0 + vf * (L::KV_BYTES / 16);
+                    const uint64_t dv = dv0 + vf * (L::KV_BYTES / 16);
+                    if (i < c) {
                         ok = wait_b(&p_full[t * NS + b], (pp >> b) & 1, s_abort, a.err, 35) && ok;
                         pp ^= 1u << b;
-                        tc_after();
+                    }
+                    if (i + NS < n) keys();
+                    my_turn();
+                    tc_after();
+                    if (i < c) {  // O += P V
 #pragma unroll
                         for (int kk = 0; kk < KS / 16; kk++)
                             mma_ts(lead && ok, d_o, d_s + b * KS + kk * 8, dv + kk * 128, id_o, i > 0 || kk ? 1u : 0u);
+                        if (NS > 1 || i == c - 1) commit(lead, &o_full[t]);
                     }
-                    if (i < c && (NS > 1 || i == c - 1)) commit(lead, &o_full[t]);
                     if (i + NS < n) {
                         scores(i + NS);
                         if (i + NS < c) commit(lead, &s_full[t * NS + b]);
-                        behind(i + NS);
                     }
+                    your_turn();
+                    if (i + NS < n) behind(i + NS);
                     commit(lead, &kv_empty[vf]);
                     step(vf, vp);
                 }
