@@ -312,18 +312,19 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
                 __threadfence();
                 for (int idx = tid; idx < nrows * (D / 4); idx += NW * 32) {
                     const int row = idx / (D / 4), d = idx % (D / 4) * 4;
+                    // (the loads of a pass do not wait for one another)
+                    auto part_c = [&](int c) { return a.part + (int64_t)(c * 2 + (c == first ? 1 : 0)) * part_floats(D); };
                     float mr = -INFINITY, lr = 0.f;
+#pragma unroll 8
+                    for (int c = first; c <= last; c++) mr = fmaxf(mr, __ldcg(part_c(c) + row * 2));
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
                     for (int c = first; c <= last; c++) {
-                        const float *p = a.part + (int64_t)(c * 2 + (c == first ? 1 : 0)) * part_floats(D);
-                        const float mw = __ldcg(p + row * 2), lw = __ldcg(p + row * 2 + 1);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p + ROWS * 2 + row * D + d));
-                        const float mn = fmaxf(mr, mw);
-                        const float fo = mr == -INFINITY ? 0.f : ex2(mr - mn), fn = mw == -INFINITY ? 0.f : ex2(mw - mn);
-                        lr = lr * fo + lw * fn;
-                        acc.x = acc.x * fo + v.x * fn, acc.y = acc.y * fo + v.y * fn;
-                        acc.z = acc.z * fo + v.z * fn, acc.w = acc.w * fo + v.w * fn;
-                        mr = mn;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_c(c) + row * 2));
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_c(c) + ROWS * 2 + row * D + d));
+                        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - mr);
+                        lr += f * ml.y;
+                        acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
                     }
                     store(row, d, acc, mr, lr);
                 }

@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
     }
     if (a.sigmoid) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) p[i] = __fdiv_rn(1.0f, 1.0f + expf(-p[i]));
+        for (int i = 0; i < PER; i++) p[i] = __frcp_rn(1.0f + expf(-p[i]));
     } else {
 #pragma unroll
         for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(FULL, mx, o));
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
         }
         __syncwarp();
         // 2^m lanes a group scan its scores for the two best
-        const int size = a.E / a.groups;
+        const int size = a.E / a.groups, shift = (size & (size - 1)) ? -1 : 31 - __clz(size);
         int lg = 32;
         while (lg * a.groups > 32) lg >>= 1;
         const int g = lane / lg, sub = lane & (lg - 1);
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int e = lane + 32 * i;
-            key[i] = e >= a.E ? 0u : (kept >> (e / size * lg)) & 1u ? ordered(kb[e]) : ordered(-INFINITY);
+            key[i] = e >= a.E ? 0u : (kept >> ((shift >= 0 ? e >> shift : e / size) * lg)) & 1u ? ordered(kb[e]) : ordered(-INFINITY);
         }
     } else {
 #pragma unroll
@@ -322,23 +322,50 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
             key[i] = e >= a.E ? 0u : ordered(a.bias ? p[i] + a.bias[e] : p[i]);
         }
     }
+    // The lane's keys in descending order, ties to the lower index (an insertion sort of
+    // the registers: a strict comparison keeps equal keys in place), so that a round of
+    // the selection only looks at the lanes' first ones.
+    uint32_t at[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) at[i] = i;
+    if (PER <= 8) {
+#pragma unroll
+        for (int i = 1; i < PER; i++)
+#pragma unroll
+            for (int j = i; j > 0; j--) {
+                const bool swap = key[j] > key[j - 1];
+                const uint32_t hk = swap ? key[j] : key[j - 1], lk = swap ? key[j - 1] : key[j];
+                const uint32_t ha = swap ? at[j] : at[j - 1], la = swap ? at[j - 1] : at[j];
+                const float hp = swap ? p[j] : p[j - 1], lp = swap ? p[j - 1] : p[j];
+                key[j - 1] = hk, key[j] = lk, at[j - 1] = ha, at[j] = la, p[j - 1] = hp, p[j] = lp;
+            }
+    }
     int my_e = 0;
     float my_w = 0.f, tot = 0.f;
     for (int c = 0; c < a.k; c++) {
-        uint32_t best = 0;
-        int at = 0;
-        float bp = 0.f;
+        uint32_t best = key[0], e0 = lane + 32 * at[0];
+        float bp = p[0];
+        if (PER > 8) {
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (key[i] > best) best = key[i], at = lane + 32 * i, bp = p[i];
+            for (int i = 1; i < PER; i++)
+                if (key[i] > best) best = key[i], e0 = lane + 32 * i, bp = p[i];
+        }
         const uint32_t top = __reduce_max_sync(FULL, best);
-        const uint32_t e = __reduce_min_sync(FULL, best == top ? (uint32_t)at : 0xffffffffu);
+        const uint32_t e = __reduce_min_sync(FULL, best == top ? e0 : 0xffffffffu);
         const float w = __shfl_sync(FULL, bp, e & 31);
         if (lane == c) my_e = (int)e, my_w = w;
         tot += w;
+        if (PER <= 8) {
+            if (e0 == e) {  // the owner's next key moves up
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            if (lane + 32 * i == (int)e) key[i] = 0u;
+                for (int i = 0; i + 1 < PER; i++) key[i] = key[i + 1], at[i] = at[i + 1], p[i] = p[i + 1];
+                key[PER - 1] = 0u;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < PER; i++)
+                if (lane + 32 * i == (int)e) key[i] = 0u;
+        }
     }
     if (lane < a.k) {
         if (a.norm) my_w = tot > 0.f ? my_w / tot : 0.f;

@@ -209,6 +209,25 @@ bool heads_ok(const at::Tensor &t, const kq_paged_cache &c, int dev) {
            dense(t, 2) && st(t, 0) % 8 == 0 && st(t, 1) % 8 == 0 && !(reinterpret_cast<uintptr_t>(t.data_ptr()) & 15);
 }
 
+// Tensors that share one allocation: a caching-allocator round trip costs the host as
+// much as the rest of such a call, and these outputs live and die together.
+struct Block {
+    at::Tensor all;
+    int64_t at = 0;
+    Block(const at::Tensor &like, int64_t bytes) : all(at::empty({bytes}, like.options().dtype(at::kByte))) {}
+    static int64_t room(int64_t n, int64_t size) { return (n * size + 15) / 16 * 16; }
+    at::Tensor take(at::IntArrayRef sizes, at::ScalarType type) {
+        int64_t n = 1;
+        for (auto v : sizes) n *= v;
+        const int64_t size = (int64_t)c10::elementSize(type);
+        auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(), c10::scalarTypeToTypeMeta(type));
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        t.unsafeGetTensorImpl()->set_storage_offset(at / size);
+        at += room(n, size);
+        return t;
+    }
+};
+
 at::Tensor stream_workspace(int dev, cudaStream_t s, size_t bytes) { return workspace(dev, reinterpret_cast<int64_t>(s), (int64_t)bytes); }
 
 py::object paged_plan(const at::Tensor &ctx, const at::Tensor &qlen, const at::Tensor &table, const at::Tensor &free_pages,
@@ -219,9 +238,9 @@ py::object paged_plan(const at::Tensor &ctx, const at::Tensor &qlen, const at::T
     const int64_t b = ctx.size(0);
     if (!vec(qlen, b, at::kInt, dev) || !vec(free_pages, -1, at::kInt, dev) || !table_ok(table, b, dev)) return py::none();
     c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-    const auto i32 = ctx.options();
-    at::Tensor cu = at::empty({b + 1}, i32), seq = at::empty({b}, i32), slots = at::empty({tokens}, i32.dtype(at::kLong)),
-               pos = at::empty({tokens}, i32), used = at::empty({1}, i32);
+    Block m(ctx, Block::room(b + 1, 4) + Block::room(b, 4) + Block::room(tokens, 8) + Block::room(tokens, 4) + 16);
+    at::Tensor cu = m.take({b + 1}, at::kInt), seq = m.take({b}, at::kInt), slots = m.take({tokens}, at::kLong),
+               pos = m.take({tokens}, at::kInt), used = m.take({1}, at::kInt);
     cudaStream_t s = at::cuda::getCurrentCUDAStream(dev).stream();
     at::Tensor ws = stream_workspace(dev, s, 256);
     const int rc = g_plan(ctx.data_ptr<int>(), qlen.data_ptr<int>(), b, table.data_ptr<int>(), table_stride(table), table.size(1),
@@ -282,7 +301,8 @@ py::object moe_route(const at::Tensor &logits, int64_t k, int64_t scoring, const
     const int64_t t = logits.size(0), e = logits.size(1);
     if (code < 0 || !dense(logits, 1) || (bias && !vec(*bias, e, at::kFloat, dev))) return py::none();
     c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-    at::Tensor idx = at::empty({t, k}, logits.options().dtype(at::kInt)), w = at::empty({t, k}, logits.options().dtype(at::kFloat));
+    Block m(logits, 2 * Block::room(t * k, 4));
+    at::Tensor idx = m.take({t, k}, at::kInt), w = m.take({t, k}, at::kFloat);
     cudaStream_t s = at::cuda::getCurrentCUDAStream(dev).stream();
     const int rc = g_route(logits.data_ptr(), code, t, e, st(logits, 0), (int)k, (int)scoring, bias ? bias->data_ptr<float>() : nullptr,
                            (int)n_groups, (int)topk_groups, norm, (float)scale, idx.data_ptr<int>(), w.data_ptr<float>(), s);
