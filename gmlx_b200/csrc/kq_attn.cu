@@ -36,11 +36,6 @@ template <int D> struct RL {
 // 1 for one that goes on in the next.
 __host__ __device__ constexpr int part_floats(int D) { return ROWS * (D + 2); }
 
-struct Tile {  // a row tile of the line of units
-    int b, h, rt, lo, hi, tiles, lo_tile;
-    int64_t u0;  // its first unit
-};
-
 // Units of one (row tile, kv head) of a request, the same for all of its row
 // tiles; a request without keys still has one, which writes its empty rows.
 __device__ __forceinline__ int tile_units(const AttnArgs &a, const Request &r, int &lo_tile) {
@@ -49,50 +44,59 @@ __device__ __forceinline__ int tile_units(const AttnArgs &a, const Request &r, i
     lo_tile = lo / KT;
     return max(1, (hi + KT - 1) / KT - lo_tile);
 }
-__device__ __forceinline__ int64_t request_units(const AttnArgs &a, const Request &r) {
+template <class U> __device__ __forceinline__ U request_units(const AttnArgs &a, const Request &r) {
     const int64_t rows = (int64_t)r.n * a.G;
     if (rows == 0 || rows > a.max_rows || rows < a.min_rows) return 0;
     int lt;
-    return (int64_t)((rows + ROWS - 1) / ROWS) * a.Hk * tile_units(a, r, lt);
+    return (U)((rows + ROWS - 1) / ROWS) * (U)a.Hk * (U)tile_units(a, r, lt);
 }
+// token of a packed row (G divides without a division where it can)
+__device__ __forceinline__ int row_token(const AttnArgs &a, int r) { return a.g_shift >= 0 ? r >> a.g_shift : r / a.G; }
 
-template <bool F16, int D>
-__global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
+template <bool F16, int D, class U>
+__global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_constant__ AttnArgs a) {
     using L = RL<D>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t s_warp[NW], s_before;
-    __shared__ int s_run, s_last;
+    __shared__ U s_warp[NW], s_before;
+    __shared__ int s_b, s_last;
+    __shared__ Request s_rq;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     bool bad = false, bad_page = false;
 
     // units of each thread's run of requests (b == B: the padding tokens)
     const int nb = a.B + 1, per = (nb + NW * 32 - 1) / (NW * 32);
-    int64_t mine = 0;
+    U mine = 0;
+    Request rq;
     for (int i = 0; i < per; i++) {
         const int b = tid * per + i;
-        if (b < nb) mine += request_units(a, load_request(a, b, bad));
+        if (b < nb) mine += request_units<U>(a, rq = load_request(a, b, bad));
     }
-    int64_t total;
-    const int64_t upto = block_scan<NW * 32>(mine, s_warp, total);
+    U total;
+    const U upto = block_scan<NW * 32, U>(mine, s_warp, total);
     // at most one block a unit, so that the blocks of a row tile are neighbours
-    const int grid = (int)min((int64_t)gridDim.x, total);
+    const int grid = (int)min((U)gridDim.x, total);
     if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
     if ((int)blockIdx.x >= grid) return;
-    const int64_t ub = unit_begin(total, blockIdx.x, grid), ue = unit_begin(total, blockIdx.x + 1, grid);
+    const U ub = unit_begin<U>(total, blockIdx.x, grid), ue = unit_begin<U>(total, blockIdx.x + 1, grid);
 
     // the request that holds unit ub
-    if (upto - mine <= ub && ub < upto) s_run = tid, s_before = upto - mine;
-    __syncthreads();
-    int b = s_run * per;
-    int64_t before = s_before;  // units before request b
-    Request rq = load_request(a, b, bad);
-    for (;;) {
-        const int64_t n = request_units(a, rq);
-        if (ub < before + n) break;
-        before += n;
-        rq = load_request(a, ++b, bad);
+    if (upto - mine <= ub && ub < upto) {
+        U before = upto - mine;
+        int b = tid * per;
+        if (per > 1)
+            for (;; b++) {
+                rq = load_request(a, b, bad);
+                const U n = request_units<U>(a, rq);
+                if (ub < before + n) break;
+                before += n;
+            }
+        s_b = b, s_before = before, s_rq = rq;
     }
+    __syncthreads();
+    int b = s_b;
+    U before = s_before;  // units before request b
+    rq = s_rq;
 
     const uint32_t ring = smem_u32(smem) + warp * L::WARP;
     const uint16_t *kc = reinterpret_cast<const uint16_t *>(a.kc), *vc = reinterpret_cast<const uint16_t *>(a.vc);
@@ -100,22 +104,22 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
     const float sl2 = a.scale * LOG2E;
     const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
 
-    for (int64_t u = ub; u < ue;) {
-        int64_t units = request_units(a, rq);
+    for (U u = ub; u < ue;) {
+        U units = request_units<U>(a, rq);
         while (u >= before + units) {
             before += units;
             rq = load_request(a, ++b, bad);
-            units = request_units(a, rq);
+            units = request_units<U>(a, rq);
         }
         int lo_tile;
         const int tiles = tile_units(a, rq, lo_tile);
-        const int64_t item = (u - before) / tiles;
-        const int64_t u0 = before + item * tiles;  // first unit of this row tile
-        const int h = (int)(item % a.Hk), rt = (int)(item / a.Hk);
-        const int k0 = (int)(u - u0), k1 = (int)min((int64_t)tiles, ue - u0);
+        const U item = (u - before) / (U)tiles;
+        const U u0 = before + item * (U)tiles;  // first unit of this row tile
+        const int rt = (int)(item / (U)a.Hk), h = (int)(item - (U)rt * (U)a.Hk);
+        const int k0 = (int)(u - u0), k1 = (int)min((U)tiles, ue - u0);
         u = u0 + k1;
         const int nrows = min(ROWS, rq.n * a.G - rt * ROWS);
-        const int t0 = rt * ROWS / a.G, t1 = (rt * ROWS + nrows - 1) / a.G + 1;
+        const int t0 = row_token(a, rt * ROWS), t1 = row_token(a, rt * ROWS + nrows - 1) + 1;
         int lo, hi;
         key_range(a, rq, t0, t1, lo, hi);
 
@@ -125,11 +129,11 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
         const uint16_t *qp[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-            const int r = rt * ROWS + gr + 8 * i, tok = r / a.G;
+            const int r = rt * ROWS + gr + 8 * i, tok = row_token(a, r);
             const bool live = gr + 8 * i < nrows;
             lim[i] = !live ? 0 : a.causal ? rq.len - rq.n + tok + 1 : rq.len;
             low[i] = a.window ? lim[i] - a.window : 0;
-            qp[i] = live ? reinterpret_cast<const uint16_t *>(a.q) + (rq.q0 + tok) * a.q_ts + (int64_t)(h * a.G + r % a.G) * a.q_hs
+            qp[i] = live ? reinterpret_cast<const uint16_t *>(a.q) + (rq.q0 + tok) * a.q_ts + (int64_t)(h * a.G + r - tok * a.G) * a.q_hs
                          : nullptr;
         }
 #pragma unroll
@@ -269,13 +273,14 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
                         make_float2(o[j][2 * i], o[j][2 * i + 1]);
         __syncthreads();
 
-        const int first = unit_block(total, u0, grid), last = unit_block(total, u0 + tiles - 1, grid);
+        const int first = unit_block<U>(total, u0, grid), last = unit_block<U>(total, u0 + tiles - 1, grid);
         const bool split = first != last;
         float *part = a.part + (int64_t)(blockIdx.x * 2 + (k0 == 0 ? 1 : 0)) * part_floats(D);
         auto store = [&](int row, int d, float4 v, float mr, float lr) {
             const int r = rt * ROWS + row;
             const float inv = lr > 0.f ? 1.0f / lr : 0.f;
-            const int64_t orow = (int64_t)(rq.q0 + r / a.G) * a.Hq + h * a.G + r % a.G;
+            const int tok = row_token(a, r);
+            const int64_t orow = (int64_t)(rq.q0 + tok) * a.Hq + h * a.G + r - tok * a.G;
             uint2 w = make_uint2(pack_half<F16>(v.x * inv, v.y * inv), pack_half<F16>(v.z * inv, v.w * inv));
             *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + d) = w;
             if (d == 0 && a.lse) a.lse[orow] = lr > 0.f ? mr * LN2 + logf(lr) : -INFINITY;
@@ -300,31 +305,43 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
             }
         }
         if (split) {
-            __threadfence();
             __syncthreads();
-            if (tid == 0) {
-                const int n = atomicAdd(a.cnt + first, 1);
+            if (tid == 0) {  // releases the block's rows (ordered before it by the barrier), and acquires the others'
+                int n;
+                asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;" : "=r"(n) : "l"(a.cnt + first) : "memory");
                 s_last = n == last - first;
                 if (s_last) a.cnt[first] = 0;
             }
             __syncthreads();
             if (s_last) {
-                __threadfence();
+                constexpr int BATCH = 8;  // parts whose loads are under way together
                 for (int idx = tid; idx < nrows * (D / 4); idx += NW * 32) {
                     const int row = idx / (D / 4), d = idx % (D / 4) * 4;
-                    // (the loads of a pass do not wait for one another)
-                    auto part_c = [&](int c) { return a.part + (int64_t)(c * 2 + (c == first ? 1 : 0)) * part_floats(D); };
                     float mr = -INFINITY, lr = 0.f;
-#pragma unroll 8
-                    for (int c = first; c <= last; c++) mr = fmaxf(mr, __ldcg(part_c(c) + row * 2));
                     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-                    for (int c = first; c <= last; c++) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part_c(c) + row * 2));
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(part_c(c) + ROWS * 2 + row * D + d));
-                        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - mr);
-                        lr += f * ml.y;
-                        acc.x += f * v.x, acc.y += f * v.y, acc.z += f * v.z, acc.w += f * v.w;
+                    for (int c0 = first; c0 <= last; c0 += BATCH) {
+                        float2 ml[BATCH];
+                        float4 v[BATCH];
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) {
+                            const int c = min(c0 + i, last);
+                            const float *p = a.part + (int64_t)(c * 2 + (c == first ? 1 : 0)) * part_floats(D);
+                            ml[i] = __ldcg(reinterpret_cast<const float2 *>(p + row * 2));
+                            v[i] = __ldcg(reinterpret_cast<const float4 *>(p + ROWS * 2 + row * D + d));
+                            if (c0 + i > last) ml[i].x = -INFINITY;
+                        }
+                        float mn = mr;
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) mn = fmaxf(mn, ml[i].x);
+                        const float fo = mr == -INFINITY ? 0.f : ex2(mr - mn);
+                        lr *= fo, acc.x *= fo, acc.y *= fo, acc.z *= fo, acc.w *= fo;
+#pragma unroll
+                        for (int i = 0; i < BATCH; i++) {
+                            const float f = ml[i].x == -INFINITY ? 0.f : ex2(ml[i].x - mn);
+                            lr += f * ml[i].y;
+                            acc.x += f * v[i].x, acc.y += f * v[i].y, acc.z += f * v[i].z, acc.w += f * v[i].w;
+                        }
+                        mr = mn;
                     }
                     store(row, d, acc, mr, lr);
                 }
@@ -335,12 +352,19 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const AttnArgs a) {
     if (bad_page) atomicCAS(a.err, 0, ERR_INDEX);
 }
 
-template <bool F16, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
+template <bool F16, int D, class U> cudaError_t launch_as(const AttnArgs &a, cudaStream_t st) {
     const int smem = RL<D>::SMEM;
-    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<F16, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<F16, D, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    rows_kernel<F16, D><<<CTAS * num_sms(), NW * 32, smem, st>>>(a);
+    rows_kernel<F16, D, U><<<CTAS * num_sms(), NW * 32, smem, st>>>(a);
     return cudaGetLastError();
+}
+
+template <bool F16, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
+    // row tiles (one more a request than whole ones) x heads x the most units of one
+    const double most = ((double)a.T * a.G / ROWS + a.B + 1) * a.Hk * ((double)a.max_len / KT + 2);
+    if (most < 1e15 && units_fit32((int64_t)most, CTAS * num_sms())) return launch_as<F16, D, uint32_t>(a, st);
+    return launch_as<F16, D, int64_t>(a, st);
 }
 
 }  // namespace

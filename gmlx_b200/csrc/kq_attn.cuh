@@ -53,38 +53,37 @@ __device__ __forceinline__ float soft_cap(float x, float in, float out) {
     return out - __fdividef(2.0f * out, 1.0f + ex2(x * (2.0f * LOG2E * in)));
 }
 
-// Where a block's run of units starts, when thread i of it counted `mine` units
-// in its run of requests: that thread and the units before it; the units in all.
-struct Start {
-    int thread;
-    int64_t before, total;
-};
-template <int N> __device__ __forceinline__ int64_t block_scan(int64_t mine, int64_t *s_warp, int64_t &total) {  // inclusive
+// Inclusive scan of a count a thread over the block, and the total.  U is 32 bits wide
+// wherever the host can bound the total (a 64-bit scan takes twice the shuffles, and a
+// 64-bit division some 400 clocks, each of them on the path of a single token).
+template <int N, class U> __device__ __forceinline__ U block_scan(U mine, U *s_warp, U &total) {
     static_assert(N % 32 == 0 && N <= 1024, "whole warps");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t v = mine;
+    U v = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, v, o);
+        const U u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
     }
     if (lane == 31) s_warp[warp] = v;
     __syncthreads();
-    int64_t w = lane < N / 32 ? s_warp[lane] : 0;
+    U w = lane < N / 32 ? s_warp[lane] : 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t u = __shfl_up_sync(0xffffffffu, w, o);
+    for (int o = 1; o < N / 32; o <<= 1) {
+        const U u = __shfl_up_sync(0xffffffffu, w, o);
         if (lane >= o) w += u;
     }
-    total = __shfl_sync(0xffffffffu, w, 31);
-    const int64_t below = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    total = __shfl_sync(0xffffffffu, w, N / 32 - 1);
+    const U below = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
     return v + (warp ? below : 0);
 }
 
 // Unit u of `total` belongs to block ((u + 1) * grid - 1) / total, when block c
 // takes the units [c * total / grid, (c + 1) * total / grid).
-__device__ __forceinline__ int64_t unit_begin(int64_t total, int c, int grid) { return total * c / grid; }
-__device__ __forceinline__ int unit_block(int64_t total, int64_t u, int grid) { return (int)(((u + 1) * grid - 1) / total); }
+template <class U> __device__ __forceinline__ U unit_begin(U total, int c, int grid) { return total * (U)c / (U)grid; }
+template <class U> __device__ __forceinline__ int unit_block(U total, U u, int grid) { return (int)(((u + 1) * (U)grid - 1) / total); }
+// Whether unit counts up to `most` may be 32 bits wide (their products with the grid too).
+inline bool units_fit32(int64_t most, int grid) { return most >= 0 && most < (int64_t)(0xffffffffu / (unsigned)grid) - 1; }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool full) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(full ? 16 : 0) : "memory");

@@ -372,7 +372,7 @@ template <int D> struct Walk {
         s.q0 = rq.q0, s.n = rq.n, s.len = rq.len, s.b = b, s.lo = lo, s.hi = hi;
         s.h = (int)((u - before) / t);
         const int64_t u0 = before + (int64_t)s.h * t;  // first unit of the pair
-        s.first = unit_block(total, u0, grid), s.last = unit_block(total, u0 + t - 1, grid);
+        s.first = unit_block<int64_t>(total, u0, grid), s.last = unit_block<int64_t>(total, u0 + t - 1, grid);
         s.tok0 = qt * NT * p.tile_tok;
         s.lo_tile = lo / KT;
         s.tiles = (hi + KT - 1) / KT - s.lo_tile;
@@ -468,14 +468,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) s_most[warp] = most;
     int64_t total, pairs;
-    int64_t upto = block_scan<THREADS>(mine, s_warp, total);
-    const int64_t items_upto = block_scan<THREADS>(items, s_warp + 32, pairs);
+    int64_t upto = block_scan<THREADS, int64_t>(mine, s_warp, total);
+    const int64_t items_upto = block_scan<THREADS, int64_t>(items, s_warp + 32, pairs);
     most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s_most[lane] : 0);
     const bool whole = p.whole && pairs <= gridDim.x && most <= (total + gridDim.x - 1) / gridDim.x + JOIN_COST;
     if (whole) total = pairs, upto = items_upto, mine = items;
     const int grid = (int)min((int64_t)gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
     const bool work = (int)blockIdx.x < grid;
-    const int64_t ub = work ? unit_begin(total, blockIdx.x, grid) : 0, ue = work ? unit_begin(total, blockIdx.x + 1, grid) : 0;
+    const int64_t ub = work ? unit_begin<int64_t>(total, blockIdx.x, grid) : 0, ue = work ? unit_begin<int64_t>(total, blockIdx.x + 1, grid) : 0;
     if (work && upto - mine <= ub && ub < upto) *s_run = tid, *s_before = upto - mine;
     tc_before();
     __syncthreads();

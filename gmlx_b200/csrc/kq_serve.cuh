@@ -72,7 +72,7 @@ struct AttnArgs {
     int64_t table_stride;
     int max_len;  // table width * page, at most 2^31 - 1
     const int32_t *seq, *cu;
-    int B, T, Hq, Hk, G, D;
+    int B, T, Hq, Hk, G, D, g_shift;  // g_shift: log2(G), or -1
     float scale, softcap;  // softcap 0: none
     int causal, window;    // window 0: none
     void *out;             // [T][Hq][D]

@@ -135,8 +135,11 @@ int kq_paged_attention(const kq_paged_cache *cache, const void *q, int64_t q_tok
     a.kc = cache->k, a.vc = cache->v;
     a.page_stride = cache->page_stride, a.row_stride = cache->row_stride, a.head_stride = cache->head_stride;
     a.page = (int)cache->page_size, a.n_pages = (int)cache->pages, a.page_shift = -1;
-    for (int s = 0; s < 31; s++)
+    a.g_shift = -1;
+    for (int s = 0; s < 31; s++) {
         if (a.page == 1 << s) a.page_shift = s;
+        if (heads / hk == 1 << s) a.g_shift = s;
+    }
     a.table = block_tables, a.table_stride = table_stride;
     const int64_t max_len = table_width * cache->page_size;
     a.max_len = (int)(max_len < MOST ? max_len : MOST);
