@@ -78,6 +78,28 @@ template <int N, class U> __device__ __forceinline__ U block_scan(U mine, U *s_w
     return v + (warp ? below : 0);
 }
 
+// The same for two counts at once.
+template <int N, class U> __device__ __forceinline__ void block_scan2(U &v, U &x, U *s_warp, U &total_v, U &total_x) {
+    static_assert(N % 32 == 0 && N <= 1024, "whole warps");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const U a = __shfl_up_sync(0xffffffffu, v, o), b = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) v += a, x += b;
+    }
+    if (lane == 31) s_warp[warp] = v, s_warp[32 + warp] = x;
+    __syncthreads();
+    U w = lane < N / 32 ? s_warp[lane] : 0, y = lane < N / 32 ? s_warp[32 + lane] : 0;
+#pragma unroll
+    for (int o = 1; o < N / 32; o <<= 1) {
+        const U a = __shfl_up_sync(0xffffffffu, w, o), b = __shfl_up_sync(0xffffffffu, y, o);
+        if (lane >= o) w += a, y += b;
+    }
+    total_v = __shfl_sync(0xffffffffu, w, N / 32 - 1), total_x = __shfl_sync(0xffffffffu, y, N / 32 - 1);
+    const U below_v = __shfl_sync(0xffffffffu, w, max(warp - 1, 0)), below_x = __shfl_sync(0xffffffffu, y, max(warp - 1, 0));
+    if (warp) v += below_v, x += below_x;
+}
+
 // Unit u of `total` belongs to block ((u + 1) * grid - 1) / total, when block c
 // takes the units [c * total / grid, (c + 1) * total / grid).
 template <class U> __device__ __forceinline__ U unit_begin(U total, int c, int grid) { return total * (U)c / (U)grid; }

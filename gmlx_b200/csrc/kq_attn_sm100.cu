@@ -53,8 +53,10 @@ template <int D> struct TL {
     static constexpr int OFF_SEG = OFF_BAR + 512;
     static constexpr int SMEM = OFF_SEG + 256 + 1024;  // slots of 64 bytes
     static constexpr int S_COL = 0, O_COL = 256;  // S buffers, then O
-    // scores run NS buffers ahead, so the fills from a P's values to their keys are live at once
-    static_assert(2 * NS <= NB, "ring");
+    // keys and values have a ring each (so that each producer sees every phase of its slots);
+    // scores run NS buffers ahead
+    static constexpr int NK = (NB + 1) / 2, NV = NB - NK;
+    static_assert(NK >= NS + 1 && NV >= 2, "rings");
     static constexpr int PART = TM * (D + 2);        // floats of a tile's partial rows
 };
 
@@ -63,7 +65,6 @@ struct TileArgs {
     int box_shift;   // log2 of a page box's rows
     int tile_tok;    // tokens a tile: 128 / G
     uint32_t q_tx;   // bytes of a tile's queries
-    int whole;       // blocks may take whole pairs (their number fits 32 bits)
 };
 
 // What the join needs of a pair that block `i` begins and others end; last == i: none.
@@ -152,15 +153,6 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-#define KQ_R32(r, o) \
-    "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7]), \
-        "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), \
-        "=r"(r[o + 15]), "=r"(r[o + 16]), "=r"(r[o + 17]), "=r"(r[o + 18]), "=r"(r[o + 19]), "=r"(r[o + 20]), "=r"(r[o + 21]), \
-        "=r"(r[o + 22]), "=r"(r[o + 23]), "=r"(r[o + 24]), "=r"(r[o + 25]), "=r"(r[o + 26]), "=r"(r[o + 27]), "=r"(r[o + 28]), \
-        "=r"(r[o + 29]), "=r"(r[o + 30]), "=r"(r[o + 31])
-#define KQ_LIST32 \
-    "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}"
-
 #define KQ_R16(r) \
     "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), \
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
@@ -177,9 +169,6 @@ __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_
 __device__ __forceinline__ void tmem_ld_c32(uint32_t addr, uint32_t *r) {  // 32 columns
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 " KQ_LIST16 ", [%16];" : KQ_R16(r) : "r"(addr));
 }
-__device__ __forceinline__ void tmem_ld_c64(uint32_t addr, uint32_t *r) {  // 64 columns
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x8.b32 " KQ_LIST32 ", [%32];" : KQ_R32(r, 0) : "r"(addr));
-}
 __device__ __forceinline__ void tmem_st_c32(uint32_t addr, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.16x256b.x4.b32 [%16], " KQ_LIST16 ";" ::KQ_U16(r), "r"(addr) : "memory");
 }
@@ -190,6 +179,12 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // orders every use of r behind the wait before it
 __device__ __forceinline__ void pin(uint32_t &r) { asm volatile("" : "+r"(r)); }
+
+// Of a thread's 16 keys 0, 1, 8, 9, 16, 17, ... (counted from its first): those below n.
+__device__ __forceinline__ uint32_t keys_below(int n) {
+    n = min(max(n, 0), 32);
+    return (1u << (n / 8 * 2 + min(n & 7, 2))) - 1;
+}
 
 // w[g] of thread q of a quad <-> w[q] of thread g
 __device__ __forceinline__ void quad_transpose(uint32_t w[4], int lane) {
@@ -235,10 +230,10 @@ __device__ __forceinline__ float max3f(uint32_t x, uint32_t y, uint32_t z) {
     return v;
 }
 
-// The larger of m and a row's values in a fragment of 64 columns.
+// The larger of m and a row's values in a fragment of 32 columns.
 __device__ __forceinline__ float largest(float m, const uint32_t *x, int row) {
 #pragma unroll
-    for (int k = 0; k < 32; k += 4) m = max3f(__float_as_uint(m), x[k + 2 * row], x[k + 2 * row + 1]);
+    for (int k = 0; k < 16; k += 4) m = max3f(__float_as_uint(m), x[k + 2 * row], x[k + 2 * row + 1]);
     return m;
 }
 
@@ -278,7 +273,7 @@ template <int C> __device__ __forceinline__ void cap_poly(uint32_t *x, float in,
 #pragma unroll
     for (int i = 0; i < C; i++) k[i] = pack2f(c[i] * out, c[i] * out);
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
+    for (int i = 0; i < 16; i += 2) {
         const uint64_t u = mul2(pack2u(x[i], x[i + 1]), pack2f(in, in)), v = mul2(u, u);
         uint64_t y = k[C - 1];
 #pragma unroll
@@ -292,7 +287,7 @@ template <int C> __device__ __forceinline__ void cap_poly(uint32_t *x, float in,
 __device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) m = max3f(__float_as_uint(m), x[i] & 0x7fffffffu, x[i + 1] & 0x7fffffffu);
+    for (int i = 0; i < 16; i += 2) m = fmaxf(m, fmaxf(fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1]))));
     if (__all_sync(0xffffffffu, m * in <= 0.4f)) {
         const float c[4] = {0.9999998807907104f, -0.33331361413002014f, 0.13270977139472961f, -0.04755360260605812f};
         cap_poly(x, in, out, c);
@@ -302,7 +297,7 @@ __device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
         cap_poly(x, in, out, c);
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), in, out));
+        for (int i = 0; i < 16; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), in, out));
     }
 }
 
@@ -314,14 +309,14 @@ struct Seg {  // 64 bytes
     int lo_tile, tiles;    // key tiles of the pair
     int k0, k1;            // this block's share of them
     int c[2];              // S buffers of each tile of rows in the share
-    int first, last;       // blocks that share the pair
+    int split, last;       // whether blocks share the pair; the last of them (known to the first)
 };
 
 template <int D> struct Walk {
     static constexpr int NT = TL<D>::NT;
     const TileArgs &p;
     bool whole;  // a pair is one unit
-    int64_t u, ue, before;
+    uint32_t ub, u, ue, before;
     Request rq;
     int b, qt;  // request, pair
     bool bad;
@@ -337,32 +332,32 @@ template <int D> struct Walk {
         return (r.n + NT * p.tile_tok - 1) / (NT * p.tile_tok);
     }
     // units and pairs of a request; `most`: the longest pair so far
-    __device__ __forceinline__ static int64_t request_units(const TileArgs &p, const Request &r, int64_t &items, int &most) {
+    __device__ __forceinline__ static uint32_t request_units(const TileArgs &p, const Request &r, uint32_t &items, int &most) {
         const int n = pairs(p, r);
-        int64_t s = 0;
+        uint32_t s = 0;
         int lo, hi;
         for (int i = 0; i < n; i++) {
             const int t = pair_units(p, r, i, lo, hi);
             s += t;
             most = max(most, t);
         }
-        items += (int64_t)n * p.a.Hk;
+        items += (uint32_t)n * p.a.Hk;
         return s * p.a.Hk;
     }
 
-    __device__ __forceinline__ Walk(const TileArgs &p, bool whole, int64_t ub, int64_t ue, int b0, int64_t before0)
-        : p(p), whole(whole), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
+    __device__ __forceinline__ Walk(const TileArgs &p, bool whole, uint32_t ub, uint32_t ue, int b0, uint32_t before0)
+        : p(p), whole(whole), ub(ub), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
         if (u < ue) rq = load_request(p.a, b, bad);
     }
-    __device__ __forceinline__ bool next(Seg &s, int64_t total, int grid) {
+    __device__ __forceinline__ bool next(Seg &s, uint32_t total, int grid) {
         if (u >= ue) return false;
         int lo, hi, t;
         for (;;) {  // the pair that holds unit u
             if (qt < pairs(p, rq)) {
                 t = pair_units(p, rq, qt, lo, hi);
                 if (whole) t = 1;
-                if (u < before + (int64_t)t * p.a.Hk) break;
-                before += (int64_t)t * p.a.Hk;
+                if (u - before < (uint32_t)t * p.a.Hk) break;
+                before += (uint32_t)t * p.a.Hk;
                 qt++;
             } else {
                 qt = 0;
@@ -370,14 +365,15 @@ template <int D> struct Walk {
             }
         }
         s.q0 = rq.q0, s.n = rq.n, s.len = rq.len, s.b = b, s.lo = lo, s.hi = hi;
-        s.h = (int)((u - before) / t);
-        const int64_t u0 = before + (int64_t)s.h * t;  // first unit of the pair
-        s.first = unit_block<int64_t>(total, u0, grid), s.last = unit_block<int64_t>(total, u0 + t - 1, grid);
+        s.h = (int)((u - before) / (uint32_t)t);
+        const uint32_t u0 = before + (uint32_t)s.h * t;  // first unit of the pair
+        s.split = u0 < ub || u0 + t > ue;
+        s.last = u0 >= ub && u0 + t > ue ? unit_block<uint64_t>(total, u0 + t - 1, grid) : 0;
         s.tok0 = qt * NT * p.tile_tok;
         s.lo_tile = lo / KT;
         s.tiles = (hi + KT - 1) / KT - s.lo_tile;
         if (hi <= lo) s.tiles = 0;
-        s.k0 = (int)(u - u0), s.k1 = (int)min((int64_t)t, ue - u0);
+        s.k0 = (int)(u - u0), s.k1 = (int)min((uint32_t)t, ue - u0);
         u = u0 + s.k1;
         if (whole) s.k1 = max(1, s.tiles);
 #pragma unroll
@@ -431,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t *kv_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *kv_empty = kv_full + NB;
     uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *v_fix = q_empty + 1;
     uint64_t *s_full = v_fix + 1, *p_full = s_full + 2;  // [buffer]
-    uint64_t *o_full = p_full + 2, *drained = o_full + 2, *turn = drained + 2;  // [tile]
+    uint64_t *o_full = p_full + 2, *drained = o_full + 2, *turn = drained + 2;  // [tile] (o_full, two buffers: [buffer])
     uint64_t *seg_full = turn + 2, *seg_empty = seg_full + SLOTS;
     Seg *segs = reinterpret_cast<Seg *>(smem + L::OFF_SEG);
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(seg_empty + SLOTS);
@@ -450,10 +446,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
+    if (warp == K_WARP && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v) : "memory");
     // units of each thread's run of requests (b == B: the padding tokens)
     bool bad = false;
     const int nb = a.B + 1, per = (nb + THREADS - 1) / THREADS;
-    int64_t mine = 0, items = 0;
+    uint32_t mine = 0, items = 0;
     int most = 0;
     for (int i = 0; i < per; i++) {
         const int b = tid * per + i;
@@ -462,27 +459,31 @@ __global__ void __launch_bounds__(THREADS, 1)
     Split *splits = reinterpret_cast<Split *>(a.part);
     if (tid == 0) splits[blockIdx.x].last = blockIdx.x;
     if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
-    int64_t *s_warp = reinterpret_cast<int64_t *>(smem);  // before the first copy arrives there
-    int *s_most = reinterpret_cast<int *>(s_warp + 64), *s_run = s_most + 32;
-    int64_t *s_before = s_warp + 96;
+    uint32_t *s_warp = reinterpret_cast<uint32_t *>(smem);  // before the first copy arrives there
+    int *s_most = reinterpret_cast<int *>(s_warp + 64);
+    uint32_t *s_start = s_warp + 96;
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) s_most[warp] = most;
-    int64_t total, pairs;
-    int64_t upto = block_scan<THREADS, int64_t>(mine, s_warp, total);
-    const int64_t items_upto = block_scan<THREADS, int64_t>(items, s_warp + 32, pairs);
+    uint32_t total, pairs, upto = mine, items_upto = items;
+    block_scan2<THREADS, uint32_t>(upto, items_upto, s_warp, total, pairs);
     most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s_most[lane] : 0);
-    const bool whole = p.whole && pairs <= gridDim.x && most <= (total + gridDim.x - 1) / gridDim.x + JOIN_COST;
+    const bool whole = pairs <= gridDim.x && most <= (int)((total + gridDim.x - 1) / gridDim.x) + JOIN_COST;
     if (whole) total = pairs, upto = items_upto, mine = items;
-    const int grid = (int)min((int64_t)gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
+    const int grid = (int)min(gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
     const bool work = (int)blockIdx.x < grid;
-    const int64_t ub = work ? unit_begin<int64_t>(total, blockIdx.x, grid) : 0, ue = work ? unit_begin<int64_t>(total, blockIdx.x + 1, grid) : 0;
-    if (work && upto - mine <= ub && ub < upto) *s_run = tid, *s_before = upto - mine;
+    const uint32_t ub = work ? (uint32_t)unit_begin<uint64_t>(total, blockIdx.x, grid) : 0;
+    const uint32_t ue = work ? (uint32_t)unit_begin<uint64_t>(total, blockIdx.x + 1, grid) : 0;
+    if (work && upto - mine <= ub && ub < upto) s_start[0] = tid, s_start[1] = upto - mine;
     tc_before();
     __syncthreads();
     tc_after();
     const uint32_t tmem = *tmem_slot;
-    const int run = work ? *s_run : 0;
-    const int64_t run_before = work ? *s_before : 0;
+    const int run = work ? (int)s_start[0] : 0;
+    const uint32_t run_before = work ? s_start[1] : 0;
+    __syncthreads();
+    // rows of a tile that no query fills: zeros, so that their scores ask for nothing
+    for (int i = tid; i < NT * (D / 64) * TM * 8; i += THREADS)
+        if ((i >> 3) % TM >= p.tile_tok * a.G) *reinterpret_cast<uint4 *>(smem + i * 16) = make_uint4(0, 0, 0, 0);
     fence_async_shared();
     __syncthreads();
 
@@ -496,7 +497,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int kv = warp == V_WARP, shift = p.box_shift, nrow = KS >> shift;
             const CUtensorMap *map = kv ? &tm_v : &tm_k;
             bool bad_page = false;
-            uint32_t fill = kv, items = 0, fixes = 0;  // keys take the even fills of the ring, values the odd ones
+            const uint32_t ring = kv ? L::NV : L::NK, slot0 = kv ? L::NK : 0;
+            uint32_t fill = 0, items = 0, fixes = 0;
             Walk<D> walk(p, whole, ub, kv ? ub : ue, run * per, run_before);
             auto hand_out = [&]() -> const Seg * {  // the next share, for everyone
                 Seg next;
@@ -531,7 +533,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                         }
                     }
                 };
-                look_up(0);
                 if (!kv) {
                     wait_b(q_empty, (items & 1) ^ 1, s_abort, a.err, 31);
                     items++;
@@ -545,10 +546,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                                     tma_3d(smem + t * L::Q_BYTES + d * TM * 128, &tm_q, d * 64, h * a.G, sp->q0 + sp->tok0 + t * p.tile_tok, q_full);
                     }
                 }
-                for (int j = 0; j < n; j++, fill += 2) {
-                    const int slot = fill % NB;
+                look_up(0);
+                for (int j = 0; j < n; j++, fill++) {
+                    const int slot = slot0 + fill % ring;
                     uint8_t *dst = smem + L::OFF_KV + slot * L::KV_BYTES;
-                    const bool ok = wait_b(&kv_empty[slot], ((fill / NB) & 1) ^ 1, s_abort, a.err, 32);
+                    const bool ok = wait_b(&kv_empty[slot], ((fill / ring) & 1) ^ 1, s_abort, a.err, 32);
                     // a page's rows that no row sees may hold anything, and 0 * NaN is NaN:
                     // such values are cleared here before the tensor core sees them
                     const int tile0 = key00 + j * KS;
@@ -582,8 +584,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             if (bad_page) atomicCAS(a.err, 0, ERR_INDEX);
             if (*s_abort)  // nothing consumes what is still in flight: let it land before the block ends
-                for (uint32_t f = fill >= 2 * NB + kv ? fill - 2 * NB : kv; f < fill; f += 2)
-                    mbar_wait(&kv_full[f % NB], (f / NB) & 1, 1u << 20);
+                for (uint32_t f = fill > ring ? fill - ring : 0; f < fill; f++)
+                    mbar_wait(&kv_full[slot0 + f % ring], (f / ring) & 1, 1u << 20);
+            if (*s_abort && !kv && items) mbar_wait(q_full, (items - 1) & 1, 1u << 20);
+            if (*s_abort && kv && fixes) mbar_wait(v_fix, (fixes - 1) & 1, 1u << 20);
         } else if (warp < MMA_WARP + NT) {
             constexpr uint32_t id_s = idesc<F16>(KS, false), id_o = idesc<F16>(D, true);
             const int t = warp - MMA_WARP;
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const bool lead = lane == 0;
             bool ok = true;
             uint32_t items = 0, pp = 0;               // pp: a parity bit for each buffer's p_full
-            uint32_t kf = 0, kp = 0, vf = 1, vp = 0;  // the ring's next fill of keys and of values, and its parity
+            uint32_t kf = 0, kp = 0, vf = L::NK, vp = 0;  // the next slots of keys and of values, and their parities
             // The tiles take turns at the tensor core.  Left alone it would mix their steps, both
             // tiles would finish together, and so would their softmaxes: tensor core and SFU
             // would work one after the other, not side by side.
@@ -605,9 +609,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (NT == 2 && lead) mbar_arrive(&turn[t ^ 1]);
                 __syncwarp();
             };
-            auto step = [](uint32_t &f, uint32_t &par) {
-                f += 2;
-                if (f >= NB) f -= NB, par ^= 1;
+            auto step_k = [&] {
+                if (++kf == L::NK) kf = 0, kp ^= 1;
+            };
+            auto step_v = [&] {
+                if (++vf == NB) vf = L::NK, vp ^= 1;
             };
             for (const Seg *sp; (sp = shares.take()) != nullptr; shares.give(lane)) {
                 const int c = __shfl_sync(0xffffffffu, sp->c[t], 0), n = __shfl_sync(0xffffffffu, max(sp->c[0], sp->c[1]), 0);
@@ -633,7 +639,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 };
                 auto behind = [&](int i) {
                     commit(lead, &kv_empty[kf]);
-                    step(kf, kp);
+                    step_k();
                     if (i == n - 1) commit(lead, q_empty);
                 };
                 for (int i = 0; i < NS && i < n; i++) {
@@ -659,7 +665,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                         for (int kk = 0; kk < KS / 16; kk++)
                             mma_ts(lead && ok, d_o, d_s + b * KS + kk * 8, dv + kk * 128, id_o, i > 0 || kk ? 1u : 0u);
-                        if (NS > 1 || i == c - 1) commit(lead, &o_full[t]);
+                        if (NS > 1 || i == c - 1) commit(lead, &o_full[t + (NS > 1 ? b : 0)]);
                     }
                     if (i + NS < n) {
                         scores(i + NS);
@@ -668,7 +674,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     your_turn();
                     if (i + NS < n) behind(i + NS);
                     commit(lead, &kv_empty[vf]);
-                    step(vf, vp);
+                    step_v();
                 }
             }
             // no arrival is on its way to shared memory when the block ends
@@ -686,28 +692,31 @@ __global__ void __launch_bounds__(THREADS, 1)
         const float cap_in = CAP ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
         const uint64_t sl2_2 = pack2f(sl2, sl2);
         uint32_t sp_bits = 0;            // a parity bit for each of the tile's s_full
-        uint32_t no = 0;                 // products that o_full has told of (NS 1: of shares)
-        auto wait_o = [&] {
-            wait_b(&o_full[t], no++ & 1, s_abort, a.err, 38);
+        // Products are told of by o_full: with one buffer the share's last one; with two each
+        // on its buffer's barrier, waited for before that buffer's next P is handed over (a
+        // wait by parity must never fall two phases behind).
+        uint32_t o_bits = 0;
+        auto wait_o = [&](int b) {
+            wait_b(&o_full[t + b], (o_bits >> b) & 1, s_abort, a.err, 38);
+            o_bits ^= 1u << b;
             __syncwarp();
             tc_after();
         };
+        // token of this thread's rows, from the tile's first
+        const int rt0 = row0 / a.G, rt1 = (row0 + 8) / a.G;
         for (const Seg *sp; t < NT && (sp = shares.take()) != nullptr; shares.give(lane)) {
             const volatile Seg &s = *sp;
             const int tok0 = s.tok0 + t * p.tile_tok, live_tok = min(s.n, tok0 + p.tile_tok);
             const int shift = s.len - s.n + 1;
             bool live[2];
-            int lim[2], low[2];
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int row = row0 + 8 * r, tok = tok0 + row / a.G;
-                live[r] = row < p.tile_tok * a.G && tok < live_tok;
-                lim[r] = a.causal ? shift + min(tok, live_tok - 1) : s.len, low[r] = a.window ? lim[r] - a.window : 0;
-            }
+            for (int r = 0; r < 2; r++) live[r] = row0 + 8 * r < p.tile_tok * a.G && tok0 + (r ? rt1 : rt0) < live_tok;
             // keys that every row of the tile sees
             const int all_hi = a.causal ? shift + tok0 : s.len, all_lo = a.window ? shift + live_tok - 1 - a.window : 0;
-            float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-            const uint32_t o_base = no;
+            float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+            int seen = 0;       // bit r: row r has seen keys
+            bool unset = true;  // some row of the warp may have seen none
+            int told = 0;  // products of this share waited for
             const int c = s.c[t], first_key = (s.lo_tile + s.k0) * KT;
             for (int i = 0; i < c; i++) {
                 const int key0 = first_key + i * KS;
@@ -716,49 +725,51 @@ __global__ void __launch_bounds__(THREADS, 1)
                 sp_bits ^= 1u << (i % NS);
                 __syncwarp();  // tensor memory is read by whole warps
                 tc_after();
-                // (a phase is told from the one before the last only by who waits for both)
-                while (NS > 1 && (int)(no - o_base) < i - 1) wait_o();
-                uint32_t x[32], pk[KS / 4];
-                auto load = [&](int g) {  // 64 columns
-                    tmem_ld_c64(s_addr + g, x);
+                if (NS > 1 && i >= NS && told < i - 1) wait_o(i % NS), told++;  // product i - 2: this S is behind it
+                uint32_t x[16], pk[KS / 4];  // (as few live registers as will do: a spill here costs a third of the speed)
+                auto load = [&](int g) {  // 32 columns
+                    tmem_ld_c32(s_addr + g, x);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 32; k++) pin(x[k]);
+                    for (int k = 0; k < 16; k++) pin(x[k]);
                     if (CAP) cap_scores(x, cap_in, cap_out);
                     if (key0 + KS > all_hi || key0 < all_lo) {
 #pragma unroll
-                        for (int k = 0; k < 32; k++) {
-                            const int key = key0 + g + q2 + k / 4 * 8 + (k & 1), r = k >> 1 & 1;
-                            x[k] = key < lim[r] && key >= low[r] ? x[k] : 0xff800000u;
+                        for (int r = 0; r < 2; r++) {  // bit e: the e-th of this thread's 8 keys
+                            const int lim = a.causal ? shift + min(tok0 + (r ? rt1 : rt0), live_tok - 1) : s.len, at = key0 + g + q2;
+                            const uint32_t seen = keys_below(lim - at) & ~keys_below(a.window ? lim - a.window - at : 0);
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                const int k = e / 2 * 4 + r * 2 + (e & 1);
+                                x[k] = seen >> e & 1 ? x[k] : 0xff800000u;
+                            }
                         }
                     }
                 };
-                // P, O and l are kept relative to `ref`: the largest score of the first keys
-                // that the row sees.  A softmax needs no more than that as long as nothing
-                // overflows, since P and f32 are floating-point: bf16 bears a sum of 2^60,
-                // f16 one of 2^13 a thread.  So the maximum of later keys is only taken when
-                // the sum of their probabilities (or the exponent of one that exp2_poly
-                // would wrap) asks for it, and then they are taken again.
+                // P, O and l are kept relative to `ref`, and a softmax does not care which
+                // as long as nothing over- or underflows, since P and f32 are floating-point:
+                // bf16 bears sums of 2^-40 to 2^60, f16 (less) needs the largest score of the
+                // first keys that the row sees, and then bears 2^13 a thread.  So scores are
+                // taken as they are (f16: relative to the first keys' maximum) until a sum, or
+                // an exponent that exp2_poly would wrap, asks for a new reference: the
+                // maximum so far.  Then they are taken again.
                 float sum[2];
-                for (bool fresh = i == 0;; fresh = false) {
+                for (bool fresh = F16 && i == 0;; fresh = false) {
                     bool again = fresh;
                     if (!fresh) {
                         uint64_t base2[2], l2[2] = {0, 0};
                         float top = 0.f;
 #pragma unroll
-                        for (int r = 0; r < 2; r++) {
-                            const float base = ref[r] == -INFINITY ? 0.f : -ref[r] * sl2;
-                            base2[r] = pack2f(base, base);
-                        }
+                        for (int r = 0; r < 2; r++) base2[r] = pack2f(-ref[r] * sl2, -ref[r] * sl2);
 #pragma unroll
-                        for (int g = 0; g < KS; g += 64) {
+                        for (int g = 0; g < KS; g += 32) {
                             load(g);
 #pragma unroll
-                            for (int k = 0; k < 16; k++) {
+                            for (int k = 0; k < 8; k++) {
                                 const int r = k & 1;
                                 uint64_t y = fma2(pack2u(x[2 * k], x[2 * k + 1]), sl2_2, base2[r]);
                                 float p0, p1;
-                                if (k % 8 < POLY) {
+                                if (k < POLY) {
                                     unpack2f(y, p0, p1);
                                     top = max3f(__float_as_uint(top), __float_as_uint(p0), __float_as_uint(p1));
                                     y = exp2_poly(y);
@@ -768,41 +779,49 @@ __global__ void __launch_bounds__(THREADS, 1)
                                 pk[g / 4 + k] = pack_half<F16>(p0, p1);  // rounded to the values' type for the product
                             }
                         }
-                        bool high = top > 100.f, none = false;
 #pragma unroll
                         for (int r = 0; r < 2; r++) {
                             float la, lb;
                             unpack2f(l2[r], la, lb);
                             sum[r] = la + lb;
-                            high |= sum[r] > (F16 ? 0x1p13f : 0x1p60f);
-                            none |= live[r] && ref[r] == -INFINITY;
                         }
-                        again = (high && (live[0] || live[1])) || none;
+                        again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p13f : 0x1p60f) || top > 100.f;
+                        if (unset)
+#pragma unroll
+                            for (int r = 0; r < 2; r++) {  // the row's sum, by its four threads
+                                float whole = sum[r] + __shfl_xor_sync(0xffffffffu, sum[r], 1);
+                                whole += __shfl_xor_sync(0xffffffffu, whole, 2);
+                                again |= !(seen >> r & 1) && whole < 0x1p-40f;
+                            }
                     }
-                    if (!__any_sync(0xffffffffu, again)) break;
-                    float to[2] = {ref[0], ref[1]};
+                    if (!__any_sync(0xffffffffu, again)) {
+                        if (unset) unset = false, seen = 3;
+                        break;
+                    }
+                    float to[2] = {seen & 1 ? ref[0] : -INFINITY, seen & 2 ? ref[1] : -INFINITY};
 #pragma unroll 1
-                    for (int g = 0; g < KS; g += 64) {
+                    for (int g = 0; g < KS; g += 32) {
                         load(g);
                         to[0] = largest(to[0], x, 0), to[1] = largest(to[1], x, 1);
                     }
+                    bool on = false;
+                    float k[2];
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
                         to[r] = fmaxf(to[r], __shfl_xor_sync(0xffffffffu, to[r], 1));
                         to[r] = fmaxf(to[r], __shfl_xor_sync(0xffffffffu, to[r], 2));
-                    }
-                    // (no way on: every row's reference is its maximum -- rows without a key so
-                    // far, or scores that overflow f32)
-                    if (!__any_sync(0xffffffffu, fresh || (live[0] && to[0] > ref[0]) || (live[1] && to[1] > ref[1]))) break;
-                    float k[2];
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        k[r] = to[r] == ref[r] || i == 0 ? 1.0f : ex2((ref[r] - to[r]) * sl2);
+                        // a row that saw no key yet has nothing but the 2^-126 of masked ones
+                        const bool set = seen >> r & 1, first = !set && to[r] > -INFINITY;
+                        on |= first || (set && to[r] > ref[r]);
+                        k[r] = first ? 0.f : set && to[r] > ref[r] ? ex2((ref[r] - to[r]) * sl2) : 1.0f;
+                        if (first || set) ref[r] = to[r], seen |= 1 << r;
                         l[r] *= k[r];
-                        ref[r] = to[r];
                     }
+                    // no way on: every row has its maximum for reference (rows without a key so
+                    // far, or scores that overflow f32)
+                    if (!__any_sync(0xffffffffu, on) && !fresh) break;
                     if (i > 0) {
-                        while (NS > 1 && (int)(no - o_base) < i) wait_o();  // the last product (NS 1: this S is behind it)
+                        if (NS > 1 && told < i) wait_o((i - 1) % NS), told++;  // the last product (NS 1: this S is behind it)
 #pragma unroll 1
                         for (int d = 0; d < D; d += 32) {
                             uint32_t o[16];
@@ -825,24 +844,23 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[t * NS + i % NS]);
             }
-            if (NS == 1 && c > 0) wait_o();
-            while (NS > 1 && (int)(no - o_base) < c) wait_o();
+            if (NS == 1 && c > 0) wait_o(0);
+            for (; NS > 1 && told < c; told++) wait_o(told % NS);
             // ---- the tile's rows, or this block's part of them
             if (tok0 >= s.n) continue;
-            const int first = s.first, last = s.last;
-            const bool split = first != last;
+            const bool split = s.split;
             float inv[2];
             int64_t orow[2];
             float *part = part_of<D>(a.part, blockIdx.x, s.k0 == 0, t);
-            if (split && tid == 0 && s.k0 == 0) splits[blockIdx.x] = Split{last, s.q0, s.n, s.tok0, s.h};
+            if (split && tid == 0 && s.k0 == 0) splits[blockIdx.x] = Split{s.last, s.q0, s.n, s.tok0, s.h};
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 const int row = row0 + 8 * r;
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                if (ref[r] == -INFINITY) l[r] = 0.f;  // no key seen: exp2_poly gave 2^-126
+                if (!(seen >> r & 1)) l[r] = 0.f;  // no key seen: the 2^-126 of exp2_poly
                 inv[r] = l[r] > 0.f ? 1.0f / l[r] : 0.f;
-                orow[r] = (int64_t)(s.q0 + tok0 + row / a.G) * a.Hq + s.h * a.G + row % a.G;
+                orow[r] = (int64_t)(s.q0 + tok0 + (r ? rt1 : rt0)) * a.Hq + s.h * a.G + row - (r ? rt1 : rt0) * a.G;
                 const float ml = ref[r] * sl2;  // log2 units
                 if (q2 == 0) {
                     if (split) part[row] = l[r] > 0.f ? ml : -INFINITY, part[TM + row] = l[r];
@@ -942,7 +960,6 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     p.box_shift = shift;
     p.tile_tok = TM / a.G;
     p.q_tx = (uint32_t)(p.tile_tok * a.G * D * 2);
-    p.whole = (int64_t)a.T * a.Hk < (1ll << 30);
     CUtensorMap mq, mk, mv;
     // a dimension of one entry has no stride of its own
     auto bytes = [](int64_t s) { return (cuuint64_t)(s > 0 ? s * 2 : 16); };
@@ -951,7 +968,9 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     const cuuint64_t cd[4] = {(cuuint64_t)D, (cuuint64_t)a.page, (cuuint64_t)a.Hk, (cuuint64_t)a.n_pages};
     const cuuint64_t cs[3] = {bytes(a.row_stride), bytes(a.head_stride), bytes(a.page_stride)};
     const cuuint32_t cb[4] = {64, 1u << shift, 1, 1};
-    taken = encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
+    // pairs (one more a request than whole ones) x heads x the most units of one
+    const double most = ((double)a.T / (L::NT * p.tile_tok) + a.B + 1) * a.Hk * ((double)a.max_len / KT + 2);
+    taken = most < 4e9 && encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
     if (!taken) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<F16, D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
     if (e != cudaSuccess) return e;
