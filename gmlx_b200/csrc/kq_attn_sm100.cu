@@ -7,7 +7,7 @@
 // which stays in TMEM.
 //
 // What bounds it: the products (a 128 x 128 x 16 step takes 64 clocks, and so does
-// one of half its width) and nearly as much time in exponentials (16 a clock and
+// one of half its width) and as much time in exponentials (16 a clock and
 // SM).  One tile's scores, softmax and product are a chain, so a block works on two
 // tiles (head dim 64, 128; S of 128 keys each): the tensor core has the one while
 // the other's softmax runs.  At 256 O takes half of TMEM, so there is one tile, and
@@ -180,7 +180,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // orders every use of r behind the wait before it
 __device__ __forceinline__ void pin(uint32_t &r) { asm volatile("" : "+r"(r)); }
 
-// Of a thread's 16 keys 0, 1, 8, 9, 16, 17, ... (counted from its first): those below n.
+// Of a thread's 8 keys 0, 1, 8, 9, ..., 25 (counted from its first): those below n.
 __device__ __forceinline__ uint32_t keys_below(int n) {
     n = min(max(n, 0), 32);
     return (1u << (n / 8 * 2 + min(n & 7, 2))) - 1;
@@ -237,31 +237,13 @@ __device__ __forceinline__ float largest(float m, const uint32_t *x, int row) {
     return m;
 }
 
-// 2^x of a pair.  The SFU gives 16 results a clock and SM, half of what the
-// tensor core's scores ask for, so POLY of 8 pairs take the FMA pipe instead:
-// x = n + f with |f| <= 1/2 (n by adding 1.5 * 2^23), 2^f by the polynomial of
-// degree 4 whose largest relative error on that interval is smallest (2.7e-6,
-// fitted by exchange of the extrema), and n added to the exponent.
-constexpr int POLY = 1;
-__device__ __forceinline__ uint64_t exp2_mufu(uint64_t x) {
+// 2^x of a pair, on the SFU.  (A share of the pairs on the FMA pipe, by a polynomial, was
+// measured: with 0, 1, 2, 3 of 8 pairs 4096 tokens on 32768 cached took 2.19, 2.20, 2.26
+// and 2.4 ms -- the issue slots are as scarce as the SFU's.)
+__device__ __forceinline__ uint64_t exp2_2(uint64_t x) {
     float u, v;
     unpack2f(x, u, v);
     return pack2f(ex2(u), ex2(v));
-}
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-    float u, v;
-    unpack2f(x, u, v);
-    x = pack2f(fmaxf(u, -126.0f), fmaxf(v, -126.0f));
-    const uint64_t big = pack2f(12582912.0f, 12582912.0f), nbig = pack2f(-12582912.0f, -12582912.0f), none = pack2f(-1.0f, -1.0f);
-    const uint64_t n = add2(x, big), f = fma2(add2(n, nbig), none, x);
-    uint64_t y = fma2(f, pack2f(0.009570102207362652f, 0.009570102207362652f), pack2f(0.05591785907745361f, 0.05591785907745361f));
-    y = fma2(y, f, pack2f(0.240247443318367f, 0.240247443318367f));
-    y = fma2(y, f, pack2f(0.6931217908859253f, 0.6931217908859253f));
-    y = fma2(y, f, pack2f(0.9999992847442627f, 0.9999992847442627f));
-    float n0, n1, y0, y1;
-    unpack2f(n, n0, n1);
-    unpack2f(y, y0, y1);
-    return pack2u(__float_as_uint(y0) + (__float_as_uint(n0) << 23), __float_as_uint(y1) + (__float_as_uint(n1) << 23));
 }
 
 // Capped scores in units of log2: out * tanh(x * in).  While |x * in| <= 1 for all of
@@ -750,15 +732,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // as long as nothing over- or underflows, since P and f32 are floating-point:
                 // bf16 bears sums of 2^-40 to 2^60, f16 (less) needs the largest score of the
                 // first keys that the row sees, and then bears 2^13 a thread.  So scores are
-                // taken as they are (f16: relative to the first keys' maximum) until a sum, or
-                // an exponent that exp2_poly would wrap, asks for a new reference: the
-                // maximum so far.  Then they are taken again.
+                // taken as they are (f16: relative to the first keys' maximum) until a sum asks
+                // for a new reference: the maximum so far.  Then they are taken again.
                 float sum[2];
                 for (bool fresh = F16 && i == 0;; fresh = false) {
                     bool again = fresh;
                     if (!fresh) {
                         uint64_t base2[2], l2[2] = {0, 0};
-                        float top = 0.f;
 #pragma unroll
                         for (int r = 0; r < 2; r++) base2[r] = pack2f(-ref[r] * sl2, -ref[r] * sl2);
 #pragma unroll
@@ -768,13 +748,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                             for (int k = 0; k < 8; k++) {
                                 const int r = k & 1;
                                 uint64_t y = fma2(pack2u(x[2 * k], x[2 * k + 1]), sl2_2, base2[r]);
-                                float p0, p1;
-                                if (k < POLY) {
-                                    unpack2f(y, p0, p1);
-                                    top = max3f(__float_as_uint(top), __float_as_uint(p0), __float_as_uint(p1));
-                                    y = exp2_poly(y);
-                                } else y = exp2_mufu(y);
+                                y = exp2_2(y);
                                 l2[r] = add2(l2[r], y);
+                                float p0, p1;
                                 unpack2f(y, p0, p1);
                                 pk[g / 4 + k] = pack_half<F16>(p0, p1);  // rounded to the values' type for the product
                             }
@@ -785,7 +761,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             unpack2f(l2[r], la, lb);
                             sum[r] = la + lb;
                         }
-                        again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p13f : 0x1p60f) || top > 100.f;
+                        again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p13f : 0x1p60f);
                         if (unset)
 #pragma unroll
                             for (int r = 0; r < 2; r++) {  // the row's sum, by its four threads
@@ -810,10 +786,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int r = 0; r < 2; r++) {
                         to[r] = fmaxf(to[r], __shfl_xor_sync(0xffffffffu, to[r], 1));
                         to[r] = fmaxf(to[r], __shfl_xor_sync(0xffffffffu, to[r], 2));
-                        // a row that saw no key yet has nothing but the 2^-126 of masked ones
                         const bool set = seen >> r & 1, first = !set && to[r] > -INFINITY;
                         on |= first || (set && to[r] > ref[r]);
-                        k[r] = first ? 0.f : set && to[r] > ref[r] ? ex2((ref[r] - to[r]) * sl2) : 1.0f;
+                        k[r] = set && to[r] > ref[r] ? ex2((ref[r] - to[r]) * sl2) : 1.0f;  // (unset: l and O are 0)
                         if (first || set) ref[r] = to[r], seen |= 1 << r;
                         l[r] *= k[r];
                     }
@@ -858,7 +833,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int row = row0 + 8 * r;
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                if (!(seen >> r & 1)) l[r] = 0.f;  // no key seen: the 2^-126 of exp2_poly
                 inv[r] = l[r] > 0.f ? 1.0f / l[r] : 0.f;
                 orow[r] = (int64_t)(s.q0 + tok0 + (r ? rt1 : rt0)) * a.Hq + s.h * a.G + row - (r ? rt1 : rt0) * a.G;
                 const float ml = ref[r] * sl2;  // log2 units
