@@ -65,6 +65,9 @@ struct TileArgs {
     int box_shift;   // log2 of a page box's rows
     int tile_tok;    // tokens a tile: 128 / G
     uint32_t q_tx;   // bytes of a tile's queries
+    // capped scores: out * tanh(x * in), and its polynomial's coefficients (in pairs) up to |x| = most
+    float cap_in, cap_out, cap_most;
+    uint64_t cap_k[4];
 };
 
 // What the join needs of a pair that block `i` begins and others end; last == i: none.
@@ -246,40 +249,26 @@ __device__ __forceinline__ uint64_t exp2_2(uint64_t x) {
     return pack2f(ex2(u), ex2(v));
 }
 
-// Capped scores in units of log2: out * tanh(x * in).  While |x * in| <= 1 for all of
-// a warp's (a score within the cap: as good as always) the tanh is an odd polynomial
-// with the smallest largest relative error (fitted by exchange of the extrema): degree
-// 11 on [0, 1], 6.7e-7; degree 7 on [0, 0.4], 1.5e-7.  That leaves the SFU alone.
-template <int C> __device__ __forceinline__ void cap_poly(uint32_t *x, float in, float out, const float (&c)[C]) {
-    uint64_t k[C];
-#pragma unroll
-    for (int i = 0; i < C; i++) k[i] = pack2f(c[i] * out, c[i] * out);
-#pragma unroll
-    for (int i = 0; i < 16; i += 2) {
-        const uint64_t u = mul2(pack2u(x[i], x[i + 1]), pack2f(in, in)), v = mul2(u, u);
-        uint64_t y = k[C - 1];
-#pragma unroll
-        for (int e = C - 2; e >= 0; e--) y = fma2(y, v, k[e]);
-        y = mul2(y, u);
-        float a, b;
-        unpack2f(y, a, b);
-        x[i] = __float_as_uint(a), x[i + 1] = __float_as_uint(b);
-    }
-}
-__device__ __forceinline__ void cap_scores(uint32_t *x, float in, float out) {
+// Capped scores in units of log2: out * tanh(x * in).  While |x * in| <= 0.4 for all of a
+// warp's (scores well within the cap: as good as always) the tanh is an odd polynomial of
+// degree 7, fitted by exchange of the extrema (largest relative error 1.5e-7), with `in`
+// and `out` in its coefficients k: x (k0 + x^2 (k1 + x^2 (k2 + x^2 k3))).
+__device__ __forceinline__ void cap_scores(uint32_t *x, const TileArgs &p) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i += 2) m = fmaxf(m, fmaxf(fabsf(__uint_as_float(x[i])), fabsf(__uint_as_float(x[i + 1]))));
-    if (__all_sync(0xffffffffu, m * in <= 0.4f)) {
-        const float c[4] = {0.9999998807907104f, -0.33331361413002014f, 0.13270977139472961f, -0.04755360260605812f};
-        cap_poly(x, in, out, c);
-    } else if (__all_sync(0xffffffffu, m * in <= 1.0f)) {
-        const float c[6] = {0.9999994039535522f, -0.3332904279232025f, 0.13281433284282684f,
-                            -0.051605675369501114f, 0.016743114218115807f, -0.003067060373723507f};
-        cap_poly(x, in, out, c);
+    if (__all_sync(0xffffffffu, m <= p.cap_most)) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const uint64_t u = pack2u(x[i], x[i + 1]), v = mul2(u, u);
+            const uint64_t y = mul2(u, fma2(v, fma2(v, fma2(v, p.cap_k[3], p.cap_k[2]), p.cap_k[1]), p.cap_k[0]));
+            float a, b;
+            unpack2f(y, a, b);
+            x[i] = __float_as_uint(a), x[i + 1] = __float_as_uint(b);
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), in, out));
+        for (int i = 0; i < 16; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), p.cap_in, p.cap_out));
     }
 }
 
@@ -313,17 +302,17 @@ template <int D> struct Walk {
         if (rows == 0 || rows > p.a.max_rows || rows < p.a.min_rows) return 0;
         return (r.n + NT * p.tile_tok - 1) / (NT * p.tile_tok);
     }
-    // units and pairs of a request; `most`: the longest pair so far
-    __device__ __forceinline__ static uint32_t request_units(const TileArgs &p, const Request &r, uint32_t &items, int &most) {
+    // units and pairs of a request (of its pairs first, first + step, ...); `most`: the longest pair so far
+    __device__ __forceinline__ static uint32_t request_units(const TileArgs &p, const Request &r, int first, int step, uint32_t &items, int &most) {
         const int n = pairs(p, r);
-        uint32_t s = 0;
+        uint32_t s = 0, k = 0;
         int lo, hi;
-        for (int i = 0; i < n; i++) {
+        for (int i = first; i < n; i += step, k++) {
             const int t = pair_units(p, r, i, lo, hi);
             s += t;
             most = max(most, t);
         }
-        items += (uint32_t)n * p.a.Hk;
+        items += k * p.a.Hk;
         return s * p.a.Hk;
     }
 
@@ -405,7 +394,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     constexpr int NT = L::NT, NB = L::NB, KS = L::KS, NS = L::NS;
     const AttnArgs &a = p.a;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset, so that it is known to be shared memory)
     uint64_t *kv_full = reinterpret_cast<uint64_t *>(smem + L::OFF_BAR), *kv_empty = kv_full + NB;
     uint64_t *q_full = kv_empty + NB, *q_empty = q_full + 1, *v_fix = q_empty + 1;
     uint64_t *s_full = v_fix + 1, *p_full = s_full + 2;  // [buffer]
@@ -432,11 +421,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     // units of each thread's run of requests (b == B: the padding tokens)
     bool bad = false;
     const int nb = a.B + 1, per = (nb + THREADS - 1) / THREADS;
+    const bool wide = nb <= THREADS / 32;  // few requests: a warp each, a lane a pair
     uint32_t mine = 0, items = 0;
     int most = 0;
     for (int i = 0; i < per; i++) {
-        const int b = tid * per + i;
-        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad), items, most);
+        const int b = wide ? warp : tid * per + i;
+        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad), wide ? lane : 0, wide ? 32 : 1, items, most);
+    }
+    if (wide) {
+        mine = __reduce_add_sync(0xffffffffu, mine), items = __reduce_add_sync(0xffffffffu, items);
+        if (lane) mine = items = 0;
     }
     Split *splits = reinterpret_cast<Split *>(a.part);
     if (tid == 0) splits[blockIdx.x].last = blockIdx.x;
@@ -460,11 +454,11 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
     tc_after();
     const uint32_t tmem = *tmem_slot;
-    const int run = work ? (int)s_start[0] : 0;
+    const int run = work ? (int)s_start[0] : 0, first_b = wide ? run >> 5 : run * per;
     const uint32_t run_before = work ? s_start[1] : 0;
     __syncthreads();
     // rows of a tile that no query fills: zeros, so that their scores ask for nothing
-    for (int i = tid; i < NT * (D / 64) * TM * 8; i += THREADS)
+    for (int i = tid; i < NT * (D / 64) * TM * 8 && p.tile_tok * a.G < TM; i += THREADS)
         if ((i >> 3) % TM >= p.tile_tok * a.G) *reinterpret_cast<uint4 *>(smem + i * 16) = make_uint4(0, 0, 0, 0);
     fence_async_shared();
     __syncthreads();
@@ -481,7 +475,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             bool bad_page = false;
             const uint32_t ring = kv ? L::NV : L::NK, slot0 = kv ? L::NK : 0;
             uint32_t fill = 0, items = 0, fixes = 0;
-            Walk<D> walk(p, whole, ub, kv ? ub : ue, run * per, run_before);
+            Walk<D> walk(p, whole, ub, kv ? ub : ue, first_b, run_before);
             auto hand_out = [&]() -> const Seg * {  // the next share, for everyone
                 Seg next;
                 if (!walk.next(next, total, grid)) next.n = 0;
@@ -501,20 +495,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (n == 0) continue;
                 const int32_t *bt = a.table + (int64_t)sp->b * a.table_stride;
                 int page[4], off[4];
-                auto look_up = [&](int j) {
+                auto look_up = [&](int j) {  // (only loads: the ids are looked at when they are used)
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const int r = lane + 32 * q, key = key00 + j * KS + (r << shift);
-                        page[q] = a.n_pages, off[q] = 0;  // out of bounds: zeros
+                        page[q] = -1, off[q] = -1;
                         if (r < nrow && key < hi && key + (1 << shift) > lo) {
                             const int col = a.page_shift >= 0 ? key >> a.page_shift : key / a.page;
-                            const int id = bt[col];
+                            page[q] = bt[col];
                             off[q] = key - col * a.page;
-                            if ((unsigned)id < (unsigned)a.n_pages) page[q] = id;
-                            else bad_page = true;
                         }
                     }
                 };
+                look_up(0);
                 if (!kv) {
                     wait_b(q_empty, (items & 1) ^ 1, s_abort, a.err, 31);
                     items++;
@@ -528,7 +521,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                                     tma_3d(smem + t * L::Q_BYTES + d * TM * 128, &tm_q, d * 64, h * a.G, sp->q0 + sp->tok0 + t * p.tile_tok, q_full);
                     }
                 }
-                look_up(0);
                 for (int j = 0; j < n; j++, fill++) {
                     const int slot = slot0 + fill % ring;
                     uint8_t *dst = smem + L::OFF_KV + slot * L::KV_BYTES;
@@ -543,10 +535,12 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         const int r = lane + 32 * q;
+                        const bool seen = off[q] >= 0, own = (unsigned)page[q] < (unsigned)a.n_pages;
+                        bad_page |= seen && !own;
                         if (r < nrow && ok)
 #pragma unroll
-                            for (int d = 0; d < D / 64; d++)
-                                tma_4d(dst + d * KS * 128 + (r << shift) * 128, map, d * 64, off[q], h, page[q], full);
+                            for (int d = 0; d < D / 64; d++)  // page n_pages is out of bounds: zeros
+                                tma_4d(dst + d * KS * 128 + (r << shift) * 128, map, d * 64, max(off[q], 0), h, seen && own ? page[q] : a.n_pages, full);
                     }
                     if (fix) {
                         wait_b(v_fix, fixes++ & 1, s_abort, a.err, 34);
@@ -671,7 +665,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t lanes = (uint32_t)((warp & 3) * 32 + (warp >> 2 & 1) * 16) << 16;
         const uint32_t o_addr = tmem + lanes + L::O_COL + t * D;
         const float sl2 = CAP ? 1.0f : a.scale * LOG2E;
-        const float cap_in = CAP ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
         const uint64_t sl2_2 = pack2f(sl2, sl2);
         uint32_t sp_bits = 0;            // a parity bit for each of the tile's s_full
         // Products are told of by o_full: with one buffer the share's last one; with two each
@@ -688,20 +681,19 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int rt0 = row0 / a.G, rt1 = (row0 + 8) / a.G;
         for (const Seg *sp; t < NT && (sp = shares.take()) != nullptr; shares.give(lane)) {
             const volatile Seg &s = *sp;
-            const int tok0 = s.tok0 + t * p.tile_tok, live_tok = min(s.n, tok0 + p.tile_tok);
-            const int shift = s.len - s.n + 1;
-            bool live[2];
-#pragma unroll
-            for (int r = 0; r < 2; r++) live[r] = row0 + 8 * r < p.tile_tok * a.G && tok0 + (r ? rt1 : rt0) < live_tok;
-            // keys that every row of the tile sees
-            const int all_hi = a.causal ? shift + tok0 : s.len, all_lo = a.window ? shift + live_tok - 1 - a.window : 0;
+            // (what only masks and the end need is read again from the slot there)
+            auto tile_tok0 = [&] { return s.tok0 + t * p.tile_tok; };
+            auto tile_end = [&] { return min(s.n, tile_tok0() + p.tile_tok); };
+            // keys that every row of the tile sees: buffers [i_lo, i_hi) need no mask
+            const int first_key = (s.lo_tile + s.k0) * KT;
+            const int all_hi = a.causal ? s.len - s.n + 1 + tile_tok0() : s.len, all_lo = a.window ? s.len - s.n + tile_end() - a.window : 0;
+            const int i_hi = (all_hi - first_key) >= 0 ? (all_hi - first_key) / KS : 0, i_lo = all_lo > first_key ? (all_lo - first_key + KS - 1) / KS : 0;
             float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
             int seen = 0;       // bit r: row r has seen keys
             bool unset = true;  // some row of the warp may have seen none
             int told = 0;  // products of this share waited for
-            const int c = s.c[t], first_key = (s.lo_tile + s.k0) * KT;
+            const int c = s.c[t];
             for (int i = 0; i < c; i++) {
-                const int key0 = first_key + i * KS;
                 const uint32_t s_addr = tmem + lanes + L::S_COL + (t * NS + i % NS) * KS;
                 wait_b(&s_full[t * NS + i % NS], (sp_bits >> (i % NS)) & 1, s_abort, a.err, 36);
                 sp_bits ^= 1u << (i % NS);
@@ -714,12 +706,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tmem_wait_ld();
 #pragma unroll
                     for (int k = 0; k < 16; k++) pin(x[k]);
-                    if (CAP) cap_scores(x, cap_in, cap_out);
-                    if (key0 + KS > all_hi || key0 < all_lo) {
+                    if (CAP) cap_scores(x, p);
+                    if (i >= i_hi || i < i_lo) {
+                        const int key0 = (s.lo_tile + s.k0) * KT + i * KS + g + q2;
 #pragma unroll
                         for (int r = 0; r < 2; r++) {  // bit e: the e-th of this thread's 8 keys
-                            const int lim = a.causal ? shift + min(tok0 + (r ? rt1 : rt0), live_tok - 1) : s.len, at = key0 + g + q2;
-                            const uint32_t seen = keys_below(lim - at) & ~keys_below(a.window ? lim - a.window - at : 0);
+                            const int lim = a.causal ? s.len - s.n + 1 + min(tile_tok0() + (r ? rt1 : rt0), tile_end() - 1) : s.len;
+                            const uint32_t seen = keys_below(lim - key0) & ~keys_below(a.window ? lim - a.window - key0 : 0);
 #pragma unroll
                             for (int e = 0; e < 8; e++) {
                                 const int k = e / 2 * 4 + r * 2 + (e & 1);
@@ -822,7 +815,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (NS == 1 && c > 0) wait_o(0);
             for (; NS > 1 && told < c; told++) wait_o(told % NS);
             // ---- the tile's rows, or this block's part of them
+            const int tok0 = tile_tok0(), live_tok = tile_end();
             if (tok0 >= s.n) continue;
+            bool live[2];
+#pragma unroll
+            for (int r = 0; r < 2; r++) live[r] = row0 + 8 * r < p.tile_tok * a.G && tok0 + (r ? rt1 : rt0) < live_tok;
             const bool split = s.split;
             float inv[2];
             int64_t orow[2];
@@ -843,32 +840,35 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             if (split && c == 0) continue;
 #pragma unroll 1
-            for (int d = 0; d < D; d += 32) {
-                uint32_t o[16];
+            for (int d = 0; d < D; d += 64) {
+                uint32_t o[32];
                 __syncwarp();
                 if (c > 0) {
                     tmem_ld_c32(o_addr + d, o);
+                    tmem_ld_c32(o_addr + d + 32, o + 16);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
+                for (int e = 0; e < 32; e++) {
                     pin(o[e]);
                     if (c == 0) o[e] = 0u;
                 }
                 if (split) {  // f32 rows behind m and l
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2)
+                    for (int e = 0; e < 32; e += 2)
                         if (live[e >> 1 & 1])
                             *reinterpret_cast<uint2 *>(part + 2 * TM + (row0 + (e >> 1 & 1) * 8) * D + d + e / 4 * 8 + q2) = make_uint2(o[e], o[e + 1]);
                 } else {
 #pragma unroll
-                    for (int r = 0; r < 2; r++) {
+                    for (int v = 0; v < 4; v++) {
+                        const int r = v & 1, half = v >> 1;
                         uint32_t w[4];
 #pragma unroll
                         for (int g = 0; g < 4; g++)
-                            w[g] = pack_half<F16>(__uint_as_float(o[g * 4 + r * 2]) * inv[r], __uint_as_float(o[g * 4 + r * 2 + 1]) * inv[r]);
+                            w[g] = pack_half<F16>(__uint_as_float(o[half * 16 + g * 4 + r * 2]) * inv[r], __uint_as_float(o[half * 16 + g * 4 + r * 2 + 1]) * inv[r]);
                         quad_transpose(w, lane);  // the quad's thread q: the 8 columns of group q
-                        if (live[r]) *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.out) + orow[r] * D + d + q2 * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+                        if (live[r])
+                            *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.out) + orow[r] * D + d + half * 32 + q2 * 4) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
                 }
             }
@@ -880,42 +880,44 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-// Joins the pair that block blockIdx.x of the tiles began and others ended: 16 of
-// its rows (blockIdx.y), 16 threads a row.
-constexpr int JOIN_ROWS = 16, JOIN_T = 256;
+// Joins the pair that block blockIdx.x of the tiles began and others ended: a share of
+// its rows (blockIdx.y), 16 threads a row.  Few blocks, since most have nothing to do.
+constexpr int JOIN_ROWS = 64, JOIN_T = 512;
 template <bool F16, int D> __global__ void __launch_bounds__(JOIN_T) join_kernel(const __grid_constant__ TileArgs p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const AttnArgs &a = p.a;
     const int first = blockIdx.x, sub = threadIdx.x & 15;
     const Split s = reinterpret_cast<const Split *>(a.part)[first];
     if (s.last == first) return;
-    const int t = blockIdx.y * JOIN_ROWS / TM, row = blockIdx.y * JOIN_ROWS % TM + (threadIdx.x >> 4);
-    const int tok = s.tok0 + t * p.tile_tok + row / a.G;
-    if (row >= p.tile_tok * a.G || tok >= min(s.n, s.tok0 + (t + 1) * p.tile_tok)) return;
-    float m = -INFINITY, l = 0.f;
+    const int t = blockIdx.y * JOIN_ROWS / TM;
+    for (int i = threadIdx.x >> 4; i < JOIN_ROWS; i += JOIN_T / 16) {
+        const int row = blockIdx.y * JOIN_ROWS % TM + i, rt = row / a.G, tok = s.tok0 + t * p.tile_tok + rt;
+        if (row >= p.tile_tok * a.G || tok >= min(s.n, s.tok0 + (t + 1) * p.tile_tok)) return;
+        float m = -INFINITY, l = 0.f;
 #pragma unroll 4
-    for (int b = first; b <= s.last; b++) m = fmaxf(m, part_of<D>(a.part, b, b == first, t)[row]);
-    float4 acc[D / 64];
+        for (int b = first; b <= s.last; b++) m = fmaxf(m, part_of<D>(a.part, b, b == first, t)[row]);
+        float4 acc[D / 64];
 #pragma unroll
-    for (int i = 0; i < D / 64; i++) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int k = 0; k < D / 64; k++) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int b = first; b <= s.last; b++) {
-        const float *q = part_of<D>(a.part, b, b == first, t);
-        const float mb = q[row], w = mb == -INFINITY ? 0.f : ex2(mb - m);
-        l += w * q[TM + row];
+        for (int b = first; b <= s.last; b++) {
+            const float *q = part_of<D>(a.part, b, b == first, t);
+            const float mb = q[row], w = mb == -INFINITY ? 0.f : ex2(mb - m);
+            l += w * q[TM + row];
 #pragma unroll
-        for (int i = 0; i < D / 64; i++) {
-            const float4 v = reinterpret_cast<const float4 *>(q + 2 * TM + row * D)[sub + i * 16];
-            if (w != 0.f) acc[i].x += w * v.x, acc[i].y += w * v.y, acc[i].z += w * v.z, acc[i].w += w * v.w;
+            for (int k = 0; k < D / 64; k++) {
+                const float4 v = reinterpret_cast<const float4 *>(q + 2 * TM + row * D)[sub + k * 16];
+                if (w != 0.f) acc[k].x += w * v.x, acc[k].y += w * v.y, acc[k].z += w * v.z, acc[k].w += w * v.w;
+            }
         }
-    }
-    const float inv = l > 0.f ? 1.0f / l : 0.f;
-    const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row % a.G;
+        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row - rt * a.G;
 #pragma unroll
-    for (int i = 0; i < D / 64; i++)
-        *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + (sub + i * 16) * 4) =
-            make_uint2(pack_half<F16>(acc[i].x * inv, acc[i].y * inv), pack_half<F16>(acc[i].z * inv, acc[i].w * inv));
-    if (sub == 0 && a.lse) a.lse[orow] = l > 0.f ? m * LN2 + logf(l) : -INFINITY;
+        for (int k = 0; k < D / 64; k++)
+            *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + (sub + k * 16) * 4) =
+                make_uint2(pack_half<F16>(acc[k].x * inv, acc[k].y * inv), pack_half<F16>(acc[k].z * inv, acc[k].w * inv));
+        if (sub == 0 && a.lse) a.lse[orow] = l > 0.f ? m * LN2 + logf(l) : -INFINITY;
+    }
 }
 
 bool encode(CUtensorMap *m, bool f16, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
@@ -934,6 +936,19 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     p.box_shift = shift;
     p.tile_tok = TM / a.G;
     p.q_tx = (uint32_t)(p.tile_tok * a.G * D * 2);
+    if (CAP) {
+        p.cap_in = a.scale / a.softcap, p.cap_out = a.softcap * LOG2E;
+        // (outside this range the powers of x or `in` could leave f32's)
+        p.cap_most = p.cap_in >= 1e-4f && p.cap_in <= 1e4f ? 0.4f / p.cap_in : -1.f;
+        const double c[4] = {0.9999998807907104, -0.33331361413002014, 0.13270977139472961, -0.04755360260605812};
+        double f = (double)p.cap_in * p.cap_out;
+        for (int i = 0; i < 4; i++, f *= (double)p.cap_in * p.cap_in) {
+            const float k = (float)(c[i] * f);
+            uint32_t bits;
+            memcpy(&bits, &k, 4);
+            p.cap_k[i] = (uint64_t)bits << 32 | bits;
+        }
+    }
     CUtensorMap mq, mk, mv;
     // a dimension of one entry has no stride of its own
     auto bytes = [](int64_t s) { return (cuuint64_t)(s > 0 ? s * 2 : 16); };
