@@ -723,46 +723,43 @@ __global__ void __launch_bounds__(THREADS, 1)
                 };
                 // P, O and l are kept relative to `ref`, and a softmax does not care which
                 // as long as nothing over- or underflows, since P and f32 are floating-point:
-                // bf16 bears sums of 2^-40 to 2^60, f16 (less) needs the largest score of the
-                // first keys that the row sees, and then bears 2^13 a thread.  So scores are
-                // taken as they are (f16: relative to the first keys' maximum) until a sum asks
-                // for a new reference: the maximum so far.  Then they are taken again.
+                // bf16 bears sums of 2^-40 to 2^60; f16 of up to 2^13 a thread, and its small
+                // values are only exact to 2^-25, so the row's largest must not be below 1 (nor
+                // is it when 64 or 128 keys sum to as much).  So scores are taken as they are
+                // until a sum asks for a new reference: the maximum so far.  Then they are
+                // taken again.
                 float sum[2];
-                for (bool fresh = F16 && i == 0;; fresh = false) {
-                    bool again = fresh;
-                    if (!fresh) {
-                        uint64_t base2[2], l2[2] = {0, 0};
+                for (;;) {
+                    uint64_t base2[2], l2[2] = {0, 0};
 #pragma unroll
-                        for (int r = 0; r < 2; r++) base2[r] = pack2f(-ref[r] * sl2, -ref[r] * sl2);
+                    for (int r = 0; r < 2; r++) base2[r] = pack2f(-ref[r] * sl2, -ref[r] * sl2);
 #pragma unroll
-                        for (int g = 0; g < KS; g += 32) {
-                            load(g);
+                    for (int g = 0; g < KS; g += 32) {
+                        load(g);
 #pragma unroll
-                            for (int k = 0; k < 8; k++) {
-                                const int r = k & 1;
-                                uint64_t y = fma2(pack2u(x[2 * k], x[2 * k + 1]), sl2_2, base2[r]);
-                                y = exp2_2(y);
-                                l2[r] = add2(l2[r], y);
-                                float p0, p1;
-                                unpack2f(y, p0, p1);
-                                pk[g / 4 + k] = pack_half<F16>(p0, p1);  // rounded to the values' type for the product
-                            }
+                        for (int k = 0; k < 8; k++) {
+                            const int r = k & 1;
+                            const uint64_t y = exp2_2(fma2(pack2u(x[2 * k], x[2 * k + 1]), sl2_2, base2[r]));
+                            l2[r] = add2(l2[r], y);
+                            float p0, p1;
+                            unpack2f(y, p0, p1);
+                            pk[g / 4 + k] = pack_half<F16>(p0, p1);  // rounded to the values' type for the product
                         }
-#pragma unroll
-                        for (int r = 0; r < 2; r++) {
-                            float la, lb;
-                            unpack2f(l2[r], la, lb);
-                            sum[r] = la + lb;
-                        }
-                        again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p13f : 0x1p60f);
-                        if (unset)
-#pragma unroll
-                            for (int r = 0; r < 2; r++) {  // the row's sum, by its four threads
-                                float whole = sum[r] + __shfl_xor_sync(0xffffffffu, sum[r], 1);
-                                whole += __shfl_xor_sync(0xffffffffu, whole, 2);
-                                again |= !(seen >> r & 1) && whole < 0x1p-40f;
-                            }
                     }
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        float la, lb;
+                        unpack2f(l2[r], la, lb);
+                        sum[r] = la + lb;
+                    }
+                    bool again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p13f : 0x1p60f);
+                    if (unset)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {  // the row's sum, by its four threads
+                            float whole = sum[r] + __shfl_xor_sync(0xffffffffu, sum[r], 1);
+                            whole += __shfl_xor_sync(0xffffffffu, whole, 2);
+                            again |= !(seen >> r & 1) && whole < (F16 ? (float)KS : 0x1p-40f);
+                        }
                     if (!__any_sync(0xffffffffu, again)) {
                         if (unset) unset = false, seen = 3;
                         break;
@@ -787,7 +784,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     }
                     // no way on: every row has its maximum for reference (rows without a key so
                     // far, or scores that overflow f32)
-                    if (!__any_sync(0xffffffffu, on) && !fresh) break;
+                    if (!__any_sync(0xffffffffu, on)) break;
                     if (i > 0) {
                         if (NS > 1 && told < i) wait_o((i - 1) % NS), told++;  // the last product (NS 1: this S is behind it)
 #pragma unroll 1
