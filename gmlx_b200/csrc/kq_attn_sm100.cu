@@ -917,9 +917,22 @@ template <bool F16, int D> __global__ void __launch_bounds__(JOIN_T) join_kernel
     }
 }
 
+// the driver's entry by name: the library itself must load on machines without a driver
+decltype(&cuTensorMapEncodeTiled) encode_fn() {
+    static decltype(&cuTensorMapEncodeTiled) fn = nullptr;
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<decltype(fn)>(p);
+    }
+    return fn;
+}
+
 bool encode(CUtensorMap *m, bool f16, int rank, const void *base, const cuuint64_t *dims, const cuuint64_t *strides, const cuuint32_t *box) {
-    cuuint32_t one[5] = {1, 1, 1, 1, 1};
-    return cuTensorMapEncodeTiled(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(base),
+    const auto fn = encode_fn();
+    const cuuint32_t one[5] = {1, 1, 1, 1, 1};
+    return fn && fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void *>(base),
                                   dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
