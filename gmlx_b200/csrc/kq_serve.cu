@@ -158,20 +158,13 @@ __global__ void __launch_bounds__(ROPE_T) rope_kernel(const RopeArgs a) {
     int pos = a.pos[t];
     int64_t slot = a.slots[t];
     bool bad = false;
-    if (pos < 0 || pos >= a.n_pos) bad = true, pos = pos < 0 ? 0 : a.n_pos - 1;
-    if (slot >= a.n_slots) bad = true, slot = -1;
     float cs[8], sn[8];
-    if (turn) {
-        const float4 *pc = reinterpret_cast<const float4 *>(a.cos + (int64_t)pos * half + c * 8);
-        const float4 *ps = reinterpret_cast<const float4 *>(a.sin + (int64_t)pos * half + c * 8);
-        *reinterpret_cast<float4 *>(cs) = pc[0], *reinterpret_cast<float4 *>(cs + 4) = pc[1];
-        *reinterpret_cast<float4 *>(sn) = ps[0], *reinterpret_cast<float4 *>(sn + 4) = ps[1];
-    }
-    const int64_t cache_row = slot < 0 ? 0 : (slot / a.page) * a.page_stride + (slot % a.page) * a.row_stride;
+    int64_t cache_row = 0;
     const uint16_t *q = reinterpret_cast<const uint16_t *>(a.q) + t * a.q_ts, *k = reinterpret_cast<const uint16_t *>(a.k) + t * a.k_ts,
                    *v = reinterpret_cast<const uint16_t *>(a.v) + t * a.v_ts;
     const int step = per * gridDim.y;
-    for (int hb = blockIdx.y * per + h0; hb < heads; hb += step * ROPE_U) {
+    const int first = blockIdx.y * per + h0;
+    for (int hb = first; hb < heads; hb += step * ROPE_U) {
         uint4 x0[ROPE_U], x1[ROPE_U];
 #pragma unroll
         for (int u = 0; u < ROPE_U; u++) {
@@ -182,6 +175,19 @@ __global__ void __launch_bounds__(ROPE_T) rope_kernel(const RopeArgs a) {
                 x0[u] = *reinterpret_cast<const uint4 *>(src + o0);
                 x1[u] = *reinterpret_cast<const uint4 *>(src + o1);
             }
+        }
+        if (hb == first) {  // what hangs on position and slot, behind loads that do not
+            if (pos < 0 || pos >= a.n_pos) bad = true, pos = pos < 0 ? 0 : a.n_pos - 1;
+            if (slot >= a.n_slots) bad = true, slot = -1;
+            if (turn) {
+                const float4 *pc = reinterpret_cast<const float4 *>(a.cos + (int64_t)pos * half + c * 8);
+                const float4 *ps = reinterpret_cast<const float4 *>(a.sin + (int64_t)pos * half + c * 8);
+                *reinterpret_cast<float4 *>(cs) = pc[0], *reinterpret_cast<float4 *>(cs + 4) = pc[1];
+                *reinterpret_cast<float4 *>(sn) = ps[0], *reinterpret_cast<float4 *>(sn + 4) = ps[1];
+            }
+            // (a 64-bit division takes some 400 clocks)
+            if (slot >> 32) cache_row = slot < 0 ? 0 : (slot / a.page) * a.page_stride + (slot % a.page) * a.row_stride;
+            else cache_row = ((uint32_t)slot / (uint32_t)a.page) * a.page_stride + ((uint32_t)slot % (uint32_t)a.page) * a.row_stride;
         }
 #pragma unroll
         for (int u = 0; u < ROPE_U; u++) {
@@ -234,11 +240,18 @@ __device__ __forceinline__ uint32_t ordered(float f) {  // NaN below everything
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__device__ __forceinline__ float load_logit(const void *p, int dtype, int64_t i) {
-    float v = dtype == F32 ? reinterpret_cast<const float *>(p)[i]
-              : dtype == BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(p)[i])
-                              : __half2float(reinterpret_cast<const __half *>(p)[i]);
-    return v != v ? -INFINITY : fminf(v, 3.402823466e38f);  // NaN: a masked expert; +inf: the largest number
+template <typename T, int PER>
+__device__ __forceinline__ void load_logits(float (&p)[PER], const RouteArgs &a, int64_t t, int lane) {
+    const T *x = reinterpret_cast<const T *>(a.logits) + t * a.stride;
+    T v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (lane + 32 * i < a.E) v[i] = x[lane + 32 * i];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const float f = lane + 32 * i < a.E ? (float)v[i] : -INFINITY;
+        p[i] = f != f ? -INFINITY : fminf(f, 3.402823466e38f);  // NaN: a masked expert; +inf: the largest number
+    }
 }
 
 constexpr int ROUTE_W = 4;  // tokens a block
@@ -253,12 +266,11 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
     float p[PER];
     uint32_t key[PER];
     float mx = -INFINITY;
+    if (a.dtype == F32) load_logits<float>(p, a, t, lane);
+    else if (a.dtype == BF16) load_logits<__nv_bfloat16>(p, a, t, lane);
+    else load_logits<__half>(p, a, t, lane);
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = lane + 32 * i;
-        p[i] = e < a.E ? load_logit(a.logits, a.dtype, t * a.stride + e) : -INFINITY;
-        mx = fmaxf(mx, p[i]);
-    }
+    for (int i = 0; i < PER; i++) mx = fmaxf(mx, p[i]);
     if (a.sigmoid) {
 #pragma unroll
         for (int i = 0; i < PER; i++) p[i] = __frcp_rn(1.0f + expf(-p[i]));
