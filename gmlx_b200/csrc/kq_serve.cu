@@ -258,7 +258,7 @@ constexpr int ROUTE_W = 4;  // tokens a block
 
 template <int PER>
 __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) {
-    extern __shared__ float s_route[];  // keys [ROUTE_W][E] (groups > 1)
+    extern __shared__ float s_route[];  // scores [ROUTE_W][E]; with groups also what the choice goes by, [ROUTE_W][E]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t = (int64_t)blockIdx.x * ROUTE_W + warp;
     if (t >= a.T) return;
@@ -290,8 +290,12 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
 #pragma unroll
         for (int i = 0; i < PER; i++) p[i] = sf > 0.f ? __fdiv_rn(p[i], sf) : 0.f;
     }
+    float *score = s_route + warp * a.E;
+#pragma unroll
+    for (int i = 0; i < PER; i++)
+        if (lane + 32 * i < a.E) score[lane + 32 * i] = p[i];
     if (a.groups > 1) {
-        float *kb = s_route + warp * a.E;
+        float *kb = score + ROUTE_W * a.E;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int e = lane + 32 * i;
@@ -348,29 +352,24 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
                 const bool swap = key[j] > key[j - 1];
                 const uint32_t hk = swap ? key[j] : key[j - 1], lk = swap ? key[j - 1] : key[j];
                 const uint32_t ha = swap ? at[j] : at[j - 1], la = swap ? at[j - 1] : at[j];
-                const float hp = swap ? p[j] : p[j - 1], lp = swap ? p[j - 1] : p[j];
-                key[j - 1] = hk, key[j] = lk, at[j - 1] = ha, at[j] = la, p[j - 1] = hp, p[j] = lp;
+                key[j - 1] = hk, key[j] = lk, at[j - 1] = ha, at[j] = la;
             }
     }
     int my_e = 0;
-    float my_w = 0.f, tot = 0.f;
     for (int c = 0; c < a.k; c++) {
         uint32_t best = key[0], e0 = lane + 32 * at[0];
-        float bp = p[0];
         if (PER > 8) {
 #pragma unroll
             for (int i = 1; i < PER; i++)
-                if (key[i] > best) best = key[i], e0 = lane + 32 * i, bp = p[i];
+                if (key[i] > best) best = key[i], e0 = lane + 32 * i;
         }
         const uint32_t top = __reduce_max_sync(FULL, best);
         const uint32_t e = __reduce_min_sync(FULL, best == top ? e0 : 0xffffffffu);
-        const float w = __shfl_sync(FULL, bp, e & 31);
-        if (lane == c) my_e = (int)e, my_w = w;
-        tot += w;
+        if (lane == c) my_e = (int)e;
         if (PER <= 8) {
             if (e0 == e) {  // the owner's next key moves up
 #pragma unroll
-                for (int i = 0; i + 1 < PER; i++) key[i] = key[i + 1], at[i] = at[i + 1], p[i] = p[i + 1];
+                for (int i = 0; i + 1 < PER; i++) key[i] = key[i + 1], at[i] = at[i + 1];
                 key[PER - 1] = 0u;
             }
         } else {
@@ -379,6 +378,10 @@ __global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) 
                 if (lane + 32 * i == (int)e) key[i] = 0u;
         }
     }
+    __syncwarp();
+    float my_w = lane < a.k ? score[my_e] : 0.f, tot = my_w;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) tot += __shfl_xor_sync(FULL, tot, o);
     if (lane < a.k) {
         if (a.norm) my_w = tot > 0.f ? my_w / tot : 0.f;
         a.idx[t * a.k + lane] = my_e;
@@ -418,7 +421,7 @@ cudaError_t launch_rope_kv_write(const RopeArgs &a, cudaStream_t st) {
 cudaError_t launch_moe_route(const RouteArgs &a, cudaStream_t st) {
     if (a.T == 0) return cudaSuccess;
     const int grid = (a.T + ROUTE_W - 1) / ROUTE_W, per = (a.E + 31) / 32;
-    const size_t smem = a.groups > 1 ? (size_t)ROUTE_W * a.E * sizeof(float) : 0;
+    const size_t smem = (size_t)ROUTE_W * a.E * sizeof(float) * (a.groups > 1 ? 2 : 1);
     if (per <= 1) route_kernel<1><<<grid, ROUTE_W * 32, smem, st>>>(a);
     else if (per <= 2) route_kernel<2><<<grid, ROUTE_W * 32, smem, st>>>(a);
     else if (per <= 4) route_kernel<4><<<grid, ROUTE_W * 32, smem, st>>>(a);
