@@ -257,7 +257,7 @@ __device__ __forceinline__ void load_logits(float (&p)[PER], const RouteArgs &a,
 constexpr int ROUTE_W = 4;  // tokens a block
 
 template <int PER>
-__global__ void __launch_bounds__(ROUTE_W * 32) route_kernel(const RouteArgs a) {
+__global__ void __launch_bounds__(ROUTE_W * 32, PER <= 8 ? 16 : 1) route_kernel(const RouteArgs a) {
     extern __shared__ float s_route[];  // scores [ROUTE_W][E]; with groups also what the choice goes by, [ROUTE_W][E]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t t = (int64_t)blockIdx.x * ROUTE_W + warp;
