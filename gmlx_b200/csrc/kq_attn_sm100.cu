@@ -75,6 +75,7 @@ struct Split {
     int last, q0, n, tok0, h;
 };
 constexpr int SPLIT_FLOATS = 8 * 256;  // room for one a block in front of the partial rows
+constexpr int PAIR_COST = 2;           // what a pair costs besides its units, in units: queries, first reference, results
 constexpr int JOIN_COST = 2;           // what a cut costs, in units: rows written, and the join's launch
 
 __device__ __forceinline__ uint64_t gtimer() {
@@ -309,7 +310,7 @@ template <int D> struct Walk {
         int lo, hi;
         for (int i = first; i < n; i += step, k++) {
             const int t = pair_units(p, r, i, lo, hi);
-            s += t;
+            s += t + PAIR_COST;
             most = max(most, t);
         }
         items += k * p.a.Hk;
@@ -322,31 +323,48 @@ template <int D> struct Walk {
     }
     __device__ __forceinline__ bool next(Seg &s, uint32_t total, int grid) {
         if (u >= ue) return false;
-        int lo, hi, t;
-        for (;;) {  // the pair that holds unit u
-            if (qt < pairs(p, rq)) {
-                t = pair_units(p, rq, qt, lo, hi);
-                if (whole) t = 1;
-                if (u - before < (uint32_t)t * p.a.Hk) break;
-                before += (uint32_t)t * p.a.Hk;
-                qt++;
+        const int lane = threadIdx.x & 31;
+        for (;;) {  // the pair that holds unit u, 32 pairs at a time
+            const int n = pairs(p, rq);
+            if (qt < n) {
+                int l, e;
+                const uint32_t cost = qt + lane < n ? (whole ? 1 : pair_units(p, rq, qt + lane, l, e) + PAIR_COST) * p.a.Hk : 0;
+                uint32_t upto = cost;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                const unsigned hit = __ballot_sync(0xffffffffu, u - before < upto);
+                if (hit) {
+                    const int j = __ffs(hit) - 1;
+                    before += __shfl_sync(0xffffffffu, upto - cost, j);
+                    qt += j;
+                    break;
+                }
+                before += __shfl_sync(0xffffffffu, upto, 31);
+                qt += 32;
             } else {
                 qt = 0;
                 rq = load_request(p.a, ++b, bad);
             }
         }
+        int lo, hi;
+        const int t = pair_units(p, rq, qt, lo, hi), tv = whole ? 1 : t + PAIR_COST;
         s.q0 = rq.q0, s.n = rq.n, s.len = rq.len, s.b = b, s.lo = lo, s.hi = hi;
-        s.h = (int)((u - before) / (uint32_t)t);
-        const uint32_t u0 = before + (uint32_t)s.h * t;  // first unit of the pair
-        s.split = u0 < ub || u0 + t > ue;
-        s.last = u0 >= ub && u0 + t > ue ? unit_block<uint64_t>(total, u0 + t - 1, grid) : 0;
+        s.h = (int)((u - before) / (uint32_t)tv);
+        const uint32_t u0 = before + (uint32_t)s.h * tv, v0 = u - u0, v1 = min((uint32_t)tv, ue - u0);
+        u = u0 + v1;
+        // The first PAIR_COST units of a pair are its fixed cost: a cut among them falls before
+        // the pair, any other before the key tile that stands there.
+        s.k0 = whole ? 0 : max(0, (int)v0 - PAIR_COST), s.k1 = whole ? t : max(0, (int)v1 - PAIR_COST);
+        if (s.k1 == 0) return false;  // (and u == ue)
+        s.split = s.k0 > 0 || s.k1 < t;
+        s.last = s.k0 == 0 && s.k1 < t ? unit_block<uint64_t>(total, u0 + tv - 1, grid) : 0;
         s.tok0 = qt * NT * p.tile_tok;
         s.lo_tile = lo / KT;
         s.tiles = (hi + KT - 1) / KT - s.lo_tile;
         if (hi <= lo) s.tiles = 0;
-        s.k0 = (int)(u - u0), s.k1 = (int)min((uint32_t)t, ue - u0);
-        u = u0 + s.k1;
-        if (whole) s.k1 = max(1, s.tiles);
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int t0 = s.tok0 + i * p.tile_tok, t1 = min(rq.n, t0 + p.tile_tok);
@@ -443,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint32_t total, pairs, upto = mine, items_upto = items;
     block_scan2<THREADS, uint32_t>(upto, items_upto, s_warp, total, pairs);
     most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s_most[lane] : 0);
-    const bool whole = pairs <= gridDim.x && most <= (int)((total + gridDim.x - 1) / gridDim.x) + JOIN_COST;
+    const bool whole = pairs <= gridDim.x && most <= (int)((total - PAIR_COST * pairs + gridDim.x - 1) / gridDim.x) + JOIN_COST;
     if (whole) total = pairs, upto = items_upto, mine = items;
     const int grid = (int)min(gridDim.x, total);  // at most one block a unit: a pair's blocks are neighbours
     const bool work = (int)blockIdx.x < grid;
@@ -967,8 +985,8 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     const cuuint64_t cd[4] = {(cuuint64_t)D, (cuuint64_t)a.page, (cuuint64_t)a.Hk, (cuuint64_t)a.n_pages};
     const cuuint64_t cs[3] = {bytes(a.row_stride), bytes(a.head_stride), bytes(a.page_stride)};
     const cuuint32_t cb[4] = {64, 1u << shift, 1, 1};
-    // pairs (one more a request than whole ones) x heads x the most units of one
-    const double most = ((double)a.T / (L::NT * p.tile_tok) + a.B + 1) * a.Hk * ((double)a.max_len / KT + 2);
+    // pairs (one more a request than whole ones) x heads x the most units of one and its fixed cost
+    const double most = ((double)a.T / (L::NT * p.tile_tok) + a.B + 1) * a.Hk * ((double)a.max_len / KT + 2 + PAIR_COST);
     taken = most < 4e9 && encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
     if (!taken) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<F16, D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
