@@ -684,6 +684,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t o_addr = tmem + lanes + L::O_COL + t * D;
         const float sl2 = CAP ? 1.0f : a.scale * LOG2E;
         const uint64_t sl2_2 = pack2f(sl2, sl2);
+        const float ref0 = F16 ? -fminf(6.f / sl2, 1e30f) : 0.f;  // f16 starts with probabilities of 2^6 times exp(score)
         uint32_t sp_bits = 0;            // a parity bit for each of the tile's s_full
         // Products are told of by o_full: with one buffer the share's last one; with two each
         // on its buffer's barrier, waited for before that buffer's next P is handed over (a
@@ -706,7 +707,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int first_key = (s.lo_tile + s.k0) * KT;
             const int all_hi = a.causal ? s.len - s.n + 1 + tile_tok0() : s.len, all_lo = a.window ? s.len - s.n + tile_end() - a.window : 0;
             const int i_hi = (all_hi - first_key) >= 0 ? (all_hi - first_key) / KS : 0, i_lo = all_lo > first_key ? (all_lo - first_key + KS - 1) / KS : 0;
-            float ref[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+            float ref[2] = {ref0, ref0}, l[2] = {0.f, 0.f};
             int seen = 0;       // bit r: row r has seen keys
             bool unset = true;  // some row of the warp may have seen none
             int told = 0;  // products of this share waited for
@@ -741,11 +742,11 @@ __global__ void __launch_bounds__(THREADS, 1)
                 };
                 // P, O and l are kept relative to `ref`, and a softmax does not care which
                 // as long as nothing over- or underflows, since P and f32 are floating-point:
-                // bf16 bears sums of 2^-40 to 2^60; f16 of up to 2^13 a thread, and its small
+                // bf16 bears sums of 2^-40 to 2^60; f16 of up to 2^15 a thread, and its small
                 // values are only exact to 2^-25, so the row's largest must not be below 1 (nor
                 // is it when 64 or 128 keys sum to as much).  So scores are taken as they are
-                // until a sum asks for a new reference: the maximum so far.  Then they are
-                // taken again.
+                // (in f16 times 2^6, halfway, which rows of few keys bear too) until a sum asks
+                // for a new reference: the maximum so far.  Then they are taken again.
                 float sum[2];
                 for (;;) {
                     uint64_t base2[2], l2[2] = {0, 0};
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         unpack2f(l2[r], la, lb);
                         sum[r] = la + lb;
                     }
-                    bool again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p13f : 0x1p60f);
+                    bool again = fmaxf(sum[0], sum[1]) > (F16 ? 0x1p15f : 0x1p60f);
                     if (unset)
 #pragma unroll
                         for (int r = 0; r < 2; r++) {  // the row's sum, by its four threads
