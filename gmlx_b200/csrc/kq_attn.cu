@@ -10,6 +10,17 @@
 // shared memory; a row tile that several blocks share goes through f32 partial
 // rows in the workspace, which the last block to arrive joins in block order
 // (so the bits do not depend on the order of arrival).
+//
+// With m the running maximum of a row's scores s_j = scale q.k_j, it keeps
+// l = sum e^(s_j - m) and o = sum e^(s_j - m) v_j; a larger maximum m' scales both
+// by e^(m - m'), two parts (m, l, o) join the same way, and the row is o / l with
+// lse = m + log l.
+// Bound: reading the cache.  64 requests on contexts of up to 16384 (8 kv heads of
+// 128, pages of 16): 1.97 GB in 298 us, 6.6 TB/s, the rate of a plain copy.  One
+// token at a context of 999 is latency: 7.5 us, of which launch, lengths, table and
+// the first keys are a chain of four round trips to memory, the join one more.
+// Above 16 rows the products would bound it (16.8 ms for 4096 tokens on 32768,
+// against 2.0 on the tensor cores).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

@@ -34,6 +34,9 @@ __device__ __forceinline__ int warp_incl_scan(int v, int lane) {
 // by a binary search in the scanned arrays: one launch, nothing between blocks.
 // A table entry that this step writes is never read by it (tokens on a new
 // page take its id from the free list), so the blocks need no order.
+// Bound: launch and latency, two dependent rounds of loads and the scan: 64
+// requests of one token 4.0 us, 1000 requests and 44,000 tokens 5.6 us, of which
+// the launch itself is some 2.3.
 constexpr int PLAN_T = 1024;
 
 __device__ __forceinline__ int upper_bound(const int *a, int n, int v) {  // entries <= v
@@ -142,7 +145,11 @@ template <> struct Half<false> {
 // interleaved one pairs neighbours, so it takes sixteen values in a row; past
 // `rot`, and for v, it copies sixteen values.  A thread keeps its place in the
 // head, and with it its eight angles, for all of its heads of a token; all of
-// its loads are issued before the first is used.
+// its loads are issued before the first is used, and what hangs on position and
+// slot (angles, the cache row) is looked up behind them.
+// Out of (a, b) come a cos - b sin and b cos + a sin, in f32 and rounded once.
+// Bound: HBM.  8192 tokens of 32 + 8 + 8 heads of 128: 206 MB in 37.0 us, 5.55 TB/s
+// (85 % of a plain copy's rate, of which 2.3 us are the launch); one token 2.3 us.
 constexpr int ROPE_T = 128, ROPE_U = 4;
 
 template <bool F16>
@@ -232,7 +239,12 @@ __global__ void __launch_bounds__(ROPE_T) rope_kernel(const RopeArgs a) {
 // functions of the logits in f32 (expf and a rounded division, the softmax's
 // sum in f64 and rounded once), so a choice never hangs on the order of a sum.
 // A float compares as the unsigned number of its ordered bits, so the best of
-// the warp is one redux.max and its lowest index one redux.min.
+// the warp is one redux.max and its lowest index one redux.min; a lane's own keys
+// are sorted first, so a round looks at one of each lane, and the scores wait in
+// shared memory for the chosen.  Bound: instructions (some 900 a warp with 256
+// experts in 8 groups), at 16 blocks an SM so that 8192 tokens are one wave:
+// 13.3 us; 64 tokens 4.9 us, one token of 128 experts 2.8 us, of which the launch
+// is 2.3 and the chain load, scores, k rounds the rest.
 
 __device__ __forceinline__ uint32_t ordered(float f) {  // NaN below everything
     const uint32_t b = __float_as_uint(f + 0.0f);
