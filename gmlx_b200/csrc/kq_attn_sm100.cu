@@ -355,7 +355,8 @@ template <int D> struct Walk {
                 qt += 32;
             } else {
                 qt = 0;
-                rq = load_request(p.a, ++b, bad);
+                if (++b > p.a.B) return false;  // (lengths that changed while they were read)
+                rq = load_request(p.a, b, bad);
             }
         }
         int lo, hi;

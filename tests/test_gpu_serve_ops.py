@@ -433,6 +433,24 @@ def test_attention_growing_maximum(cuda, lens):
         check_attn((q, kc, vc, table, seq, cu), lens[0][0])
 
 
+@pytest.mark.parametrize("d,dtype", [(64, FP), (64, BF), (128, FP), (128, BF), (256, BF)])
+@pytest.mark.parametrize("lens,window", [([(700, 700)], 0), ([(1, 40)] * 3 + [(333, 900), (90, 90), (2, 2), (400, 401)], 170)])
+def test_attention_more_pairs_than_blocks(cuda, lens, window, d, dtype):
+    """Pairs of one key tile beside pairs of many, cut wherever an even run ends."""
+    check_attn(attn_inputs(cuda, lens, 64, 8, d, 16, dtype), max(n for n, _ in lens), window=window)
+
+
+@pytest.mark.parametrize("shift", [-40.0, 40.0])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_attention_scores_far_from_zero(cuda, shift, dtype):
+    """Every score of a row near `shift`: probabilities that leave the type's range unless
+    they are taken relative to something near it."""
+    args = attn_inputs(cuda, [(150, 520), (33, 33)], 4, 2, 64, 16, dtype)
+    q, kc = args[0], args[1]
+    q[..., 0], kc[..., 0] = 8.0, torch.where(kc[..., 0].isnan(), kc[..., 0], shift)  # adds 8 shift / 8
+    check_attn(args, 150)
+
+
 @pytest.mark.parametrize("lens", [[(1, 700), (2, 30)], [(130, 700), (2, 30)]])
 def test_attention_reports_foreign_pages(cuda, lens):
     args = attn_inputs(cuda, lens, 4, 2, 128, 16, BF)
