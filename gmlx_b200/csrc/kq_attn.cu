@@ -64,7 +64,7 @@ template <class U> __device__ __forceinline__ U request_units(const AttnArgs &a,
 // token of a packed row (G divides without a division where it can)
 __device__ __forceinline__ int row_token(const AttnArgs &a, int r) { return a.g_shift >= 0 ? r >> a.g_shift : r / a.G; }
 
-template <bool F16, int D, class U>
+template <bool F16, int D, bool CAP, class U>
 __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_constant__ AttnArgs a) {
     using L = RL<D>;
     constexpr int CH = D / 8;  // 16-byte chunks of a row
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
     const uint16_t *kc = reinterpret_cast<const uint16_t *>(a.kc), *vc = reinterpret_cast<const uint16_t *>(a.vc);
     const int gr = lane >> 2, gc = lane & 3;
     const float sl2 = a.scale * LOG2E;
-    const float cap_in = a.softcap > 0.f ? a.scale / a.softcap : 0.f, cap_out = a.softcap * LOG2E;
+    const Cap cap = make_cap(a.scale, a.softcap);
 
     for (U u = ub; u < ue;) {
         U units = request_units<U>(a, rq);
@@ -209,6 +209,20 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
                     mma16816<F16>(s[1], qf[kk], kf[2], kf[3], s[1]);
                 }
             }
+            if (CAP) {
+                float far = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) far = fmaxf(far, fabsf(s[i >> 2][i & 3] * cap.in));
+                if (__all_sync(0xffffffffu, far <= CAP_NEAR))  // as good as always
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s[i >> 2][i & 3] = cap_near(s[i >> 2][i & 3], cap);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s[i >> 2][i & 3] = soft_cap(s[i >> 2][i & 3], cap);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) s[i >> 2][i & 3] *= sl2;
+            }
             const int base = (lo_tile + kt) * KT + warp * KW + gc * 2;
             float mx[2] = {m[0], m[1]};
 #pragma unroll
@@ -216,8 +230,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int key = base + j * 8 + (i & 1), row = i >> 1;
-                    const float y = a.softcap > 0.f ? soft_cap(s[j][i], cap_in, cap_out) : s[j][i] * sl2;
-                    s[j][i] = key < lim[row] && key >= low[row] ? y : -INFINITY;
+                    s[j][i] = key < lim[row] && key >= low[row] ? s[j][i] : -INFINITY;
                     mx[row] = fmaxf(mx[row], s[j][i]);
                 }
 #pragma unroll
@@ -363,19 +376,23 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
     if (bad_page) atomicCAS(a.err, 0, ERR_INDEX);
 }
 
-template <bool F16, int D, class U> cudaError_t launch_as(const AttnArgs &a, cudaStream_t st) {
+template <bool F16, int D, bool CAP, class U> cudaError_t launch_as(const AttnArgs &a, cudaStream_t st) {
     const int smem = RL<D>::SMEM;
-    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<F16, D, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const cudaError_t e = cudaFuncSetAttribute(rows_kernel<F16, D, CAP, U>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    rows_kernel<F16, D, U><<<CTAS * num_sms(), NW * 32, smem, st>>>(a);
+    rows_kernel<F16, D, CAP, U><<<CTAS * num_sms(), NW * 32, smem, st>>>(a);
     return cudaGetLastError();
 }
 
-template <bool F16, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
+template <bool F16, int D, bool CAP> cudaError_t launch_cap(const AttnArgs &a, cudaStream_t st) {
     // row tiles (one more a request than whole ones) x heads x the most units of one
     const double most = ((double)a.T * a.G / ROWS + a.B + 1) * a.Hk * ((double)a.max_len / KT + 2);
-    if (most < 1e15 && units_fit32((int64_t)most, CTAS * num_sms())) return launch_as<F16, D, uint32_t>(a, st);
-    return launch_as<F16, D, int64_t>(a, st);
+    if (most < 1e15 && units_fit32((int64_t)most, CTAS * num_sms())) return launch_as<F16, D, CAP, uint32_t>(a, st);
+    return launch_as<F16, D, CAP, int64_t>(a, st);
+}
+
+template <bool F16, int D> cudaError_t launch(const AttnArgs &a, cudaStream_t st) {
+    return a.softcap > 0.f ? launch_cap<F16, D, true>(a, st) : launch_cap<F16, D, false>(a, st);
 }
 
 }  // namespace

@@ -47,10 +47,30 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// softcap in units of log2: out * tanh(x * in), with 1 - 2 / (1 + e^2u) for the
-// tanh (the hardware's is good to 11 bits only, too few for a score of up to `cap`)
-__device__ __forceinline__ float soft_cap(float x, float in, float out) {
-    return out - __fdividef(2.0f * out, 1.0f + ex2(x * (2.0f * LOG2E * in)));
+// Capped scores in units of log2: out * tanh(u), u = x * in.  Up to |u| = CAP_NEAR the tanh
+// is an odd polynomial u (k0 + u^2 (k1 + u^2 (k2 + u^2 k3))), fitted by exchange of the
+// extrema (largest relative error 1.5e-7): there 1 - 2 / (1 + e^2u) cancels, and the score
+// would err by 2^-22 of the cap however small it is (a cap of 1e5 on scores of a few units:
+// probabilities 1.4 % off).  Beyond, 1 - 2 / (1 + e^2u) is good to some 2^-21 of itself (the
+// hardware's tanh to 2^-11 only).
+constexpr float CAP_NEAR = 0.4f;
+constexpr float CAP_K0 = 0.9999998807907104f, CAP_K1 = -0.33331361413002014f, CAP_K2 = 0.13270977139472961f,
+                CAP_K3 = -0.04755360260605812f;
+struct Cap {
+    float in, lin, out;  // lin = in * out, by itself: `in` may be too small for f32, `out` too large
+};
+__host__ __device__ __forceinline__ Cap make_cap(float scale, float softcap) {
+    // (an `in` above 1e30 belongs to a cap so small that every capped score is 0)
+    return Cap{fminf(scale / softcap, 1e30f), scale * LOG2E, softcap * LOG2E};
+}
+__device__ __forceinline__ float cap_near(float x, const Cap &c) {
+    const float u = x * c.in, v = u * u;
+    return x * c.lin * fmaf(v, fmaf(v, fmaf(v, CAP_K3, CAP_K2), CAP_K1), CAP_K0);
+}
+__device__ __forceinline__ float soft_cap(float x, const Cap &c) {
+    const float u = x * c.in;
+    if (fabsf(u) <= CAP_NEAR) return cap_near(x, c);
+    return c.out * (1.0f - __fdividef(2.0f, 1.0f + ex2(u * (2.0f * LOG2E))));
 }
 
 // Inclusive scan of a count a thread over the block, and the total.  U is 32 bits wide

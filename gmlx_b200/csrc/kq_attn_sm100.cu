@@ -73,8 +73,9 @@ struct TileArgs {
     int box_shift;   // log2 of a page box's rows
     int tile_tok;    // tokens a tile: 128 / G
     uint32_t q_tx;   // bytes of a tile's queries
-    // capped scores: out * tanh(x * in), and its polynomial's coefficients (in pairs) up to |x| = most
-    float cap_in, cap_out, cap_most;
+    // capped scores, and their polynomial's coefficients as one of x (in pairs) up to |x| = cap_most
+    Cap cap;
+    float cap_most;
     uint64_t cap_k[4];
 };
 
@@ -260,10 +261,9 @@ __device__ __forceinline__ uint64_t exp2_2(uint64_t x) {
     return pack2f(ex2(u), ex2(v));
 }
 
-// Capped scores in units of log2: out * tanh(x * in).  While |x * in| <= 0.4 for all of a
-// warp's (scores well within the cap: as good as always) the tanh is an odd polynomial of
-// degree 7, fitted by exchange of the extrema (largest relative error 1.5e-7), with `in`
-// and `out` in its coefficients k: x (k0 + x^2 (k1 + x^2 (k2 + x^2 k3))).
+// Capped scores (soft_cap).  While all of a warp's are in the polynomial's range (scores
+// well within the cap: as good as always) its coefficients k hold `in` and `out` too:
+// x (k0 + x^2 (k1 + x^2 (k2 + x^2 k3))).
 __device__ __forceinline__ void cap_scores(uint32_t *x, const TileArgs &p) {
     float m = 0.f;
 #pragma unroll
@@ -279,7 +279,7 @@ __device__ __forceinline__ void cap_scores(uint32_t *x, const TileArgs &p) {
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), p.cap_in, p.cap_out));
+        for (int i = 0; i < 16; i++) x[i] = __float_as_uint(soft_cap(__uint_as_float(x[i]), p.cap));
     }
 }
 
@@ -982,12 +982,12 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
     p.tile_tok = TM / a.G;
     p.q_tx = (uint32_t)(p.tile_tok * a.G * D * 2);
     if (CAP) {
-        p.cap_in = a.scale / a.softcap, p.cap_out = a.softcap * LOG2E;
+        p.cap = make_cap(a.scale, a.softcap);
         // (outside this range the powers of x or `in` could leave f32's)
-        p.cap_most = p.cap_in >= 1e-4f && p.cap_in <= 1e4f ? 0.4f / p.cap_in : -1.f;
-        const double c[4] = {0.9999998807907104, -0.33331361413002014, 0.13270977139472961, -0.04755360260605812};
-        double f = (double)p.cap_in * p.cap_out;
-        for (int i = 0; i < 4; i++, f *= (double)p.cap_in * p.cap_in) {
+        p.cap_most = p.cap.in >= 1e-4f && p.cap.in <= 1e4f ? CAP_NEAR / p.cap.in : -1.f;
+        const double c[4] = {CAP_K0, CAP_K1, CAP_K2, CAP_K3};
+        double f = p.cap.lin;
+        for (int i = 0; i < 4; i++, f *= (double)p.cap.in * p.cap.in) {
             const float k = (float)(c[i] * f);
             uint32_t bits;
             memcpy(&bits, &k, 4);
