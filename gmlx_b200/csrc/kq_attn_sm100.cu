@@ -995,16 +995,23 @@ template <bool F16, int D, bool CAP> cudaError_t launch(const AttnArgs &a, cudaS
         }
     }
     CUtensorMap mq, mk, mv;
-    // a dimension of one entry has no stride of its own
-    auto bytes = [](int64_t s) { return (cuuint64_t)(s > 0 ? s * 2 : 16); };
-    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.Hq, (cuuint64_t)a.T}, qs[2] = {bytes(a.q_hs), bytes(a.q_ts)};
+    // A dimension of one entry has no stride of its own; one of several entries at the same
+    // place (an expanded tensor), or at descending ones, is no map: the register tiles take
+    // any stride.
+    bool strides = true;
+    auto bytes = [&](int64_t s, int64_t extent) {
+        strides &= s > 0 || extent == 1;
+        return (cuuint64_t)(s > 0 ? s * 2 : 16);
+    };
+    const cuuint64_t qd[3] = {(cuuint64_t)D, (cuuint64_t)a.Hq, (cuuint64_t)a.T};
+    const cuuint64_t qs[2] = {bytes(a.q_hs, a.Hq), bytes(a.q_ts, a.T)};
     const cuuint32_t qb[3] = {64, (cuuint32_t)a.G, (cuuint32_t)p.tile_tok};
     const cuuint64_t cd[4] = {(cuuint64_t)D, (cuuint64_t)a.page, (cuuint64_t)a.Hk, (cuuint64_t)a.n_pages};
-    const cuuint64_t cs[3] = {bytes(a.row_stride), bytes(a.head_stride), bytes(a.page_stride)};
+    const cuuint64_t cs[3] = {bytes(a.row_stride, a.page), bytes(a.head_stride, a.Hk), bytes(a.page_stride, a.n_pages)};
     const cuuint32_t cb[4] = {64, 1u << shift, 1, 1};
     // pairs (one more a request than whole ones) x heads x the most units of one and its fixed cost
     const double most = ((double)a.T / (L::NT * p.tile_tok) + a.B + 1) * a.Hk * ((double)a.max_len / KT + 2 + PAIR_COST);
-    taken = most < 4e9 && encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
+    taken = strides && most < 4e9 && encode(&mq, F16, 3, a.q, qd, qs, qb) && encode(&mk, F16, 4, a.kc, cd, cs, cb) && encode(&mv, F16, 4, a.vc, cd, cs, cb);
     if (!taken) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(tiles_kernel<F16, D, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
     if (e != cudaSuccess) return e;

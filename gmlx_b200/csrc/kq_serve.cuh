@@ -90,7 +90,8 @@ size_t attn_tiles_part_bytes(int D);
 constexpr int ROWS_MAX = 16;
 cudaError_t launch_attn_rows(const AttnArgs &a, int dtype, cudaStream_t st);
 // Chunks (kq_attn_sm100.cu).  taken = false, nothing launched: a layout that
-// the tensor maps cannot describe, or more than 128 query heads a kv head.
+// the tensor maps cannot describe (expanded tensors among them), or more than 128
+// query heads a kv head.
 cudaError_t launch_attn_tiles(const AttnArgs &a, int dtype, cudaStream_t st, bool &taken);
 
 }  // namespace kq

@@ -1,6 +1,9 @@
 """Edges of the serving-step operators.  Tolerances are those of
 ``test_gpu_serve_ops`` (derived there)."""
 import pytest
+import torch
+
+from gmlx_b200 import kq
 
 from test_gpu_serve_ops import BF, FP, attn_inputs, check_attn
 
@@ -15,3 +18,35 @@ pytestmark = pytest.mark.gpu
                                           ([(130, 300)], 256, BF)])
 def test_caps_far_from_the_scores(cuda, lens, d, dtype, softcap):
     check_attn(attn_inputs(cuda, lens, 8, 2, d, 16, dtype), max(n for n, _ in lens), softcap=softcap)
+
+
+@pytest.mark.parametrize("what", ["cache heads", "cache rows", "cache pages", "query heads", "query tokens"])
+@pytest.mark.parametrize("lens", [[(1, 200), (3, 40)], [(150, 400), (1, 77), (40, 40)], [(60, 200)]])
+def test_expanded_tensors(cuda, lens, what):
+    """Entries that stand at the same place (stride 0): one kv head shared by all by
+    ``expand`` and the like, for chunks and single tokens alike."""
+    q, kc, vc, *rest = attn_inputs(cuda, lens, 8, 4, 128, 16, BF)
+    if what == "cache heads":
+        kc, vc = (c[:, :, 1:2].expand(-1, -1, 4, -1) for c in (kc, vc))
+    elif what == "cache rows":
+        kc, vc = (c[:, 3:4].nan_to_num(0.5).expand(-1, 16, -1, -1) for c in (kc, vc))
+    elif what == "cache pages":
+        kc, vc = (c[2:3].nan_to_num(0.5).expand(c.shape[0], -1, -1, -1) for c in (kc, vc))
+    elif what == "query heads":
+        q = q[:, 2:3].expand(-1, 8, -1)
+    else:
+        q = q[1:2].expand(q.shape[0], -1, -1)
+    assert 0 in (*q.stride(), *kc.stride())
+    check_attn((q, kc, vc, *rest), max(n for n, _ in lens))
+
+
+def test_expanded_heads_are_turned_and_stored(cuda):
+    """Queries, keys and values of one head, expanded to several: as their copies."""
+    q, k, v = (torch.randn(5, 1, 64, device=cuda).to(BF).expand(-1, h, -1) for h in (4, 2, 2))
+    angle = torch.randn(8, 32, device=cuda)
+    slots = torch.arange(5, device=cuda)
+    outs = []
+    for args in ((q, k, v), (q.contiguous(), k.contiguous(), v.contiguous())):
+        kc, vc = torch.zeros(2, 2, 4, 2, 64, device=cuda, dtype=BF)
+        outs.append((kq.rope_kv_write(*args, angle.cos(), angle.sin(), slots.int(), kc, vc, slots), kc, vc))
+    assert all(torch.equal(a, b) for a, b in zip(*outs)) and kq.workspace_error() == 0
