@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
     __shared__ int s_b, s_last;
     __shared__ Request s_rq;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    bool bad = false, bad_page = false;
+    uint32_t bad = 0;
+    bool bad_page = false;
 
     // units of each thread's run of requests (b == B: the padding tokens)
     const int nb = a.B + 1, per = (nb + NW * 32 - 1) / (NW * 32);
@@ -84,10 +85,12 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
         if (b < nb) mine += request_units<U>(a, rq = load_request(a, b, bad));
     }
     U total;
-    const U upto = block_scan<NW * 32, U>(mine, s_warp, total);
+    bool unordered = bad & BAD_ORDER;
+    const U upto = block_scan<NW * 32, U>(mine, s_warp, total, unordered);
+    if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
+    if (unordered) return write_empty(a);
     // at most one block a unit, so that the blocks of a row tile are neighbours
     const int grid = (int)min((U)gridDim.x, total);
-    if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
     if ((int)blockIdx.x >= grid) return;
     const U ub = unit_begin<U>(total, blockIdx.x, grid), ue = unit_begin<U>(total, blockIdx.x + 1, grid);
 
@@ -99,7 +102,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
             for (;; b++) {
                 rq = load_request(a, b, bad);
                 const U n = request_units<U>(a, rq);
-                if (ub < before + n) break;
+                if (ub < before + n || b == a.B) break;
                 before += n;
             }
         s_b = b, s_before = before, s_rq = rq;
@@ -117,7 +120,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
 
     for (U u = ub; u < ue;) {
         U units = request_units<U>(a, rq);
-        while (u >= before + units) {
+        while (u >= before + units && b < a.B) {
             before += units;
             rq = load_request(a, ++b, bad);
             units = request_units<U>(a, rq);

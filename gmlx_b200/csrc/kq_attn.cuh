@@ -19,10 +19,15 @@ struct Request {
     int q0, n, len;
 };
 
+// What load_request finds wrong: lengths or offsets cut to the buffers; offsets that descend.
+constexpr uint32_t BAD_CUT = 1, BAD_ORDER = 2;
+
 // Request b of the call; b == B stands for the padding tokens behind the last
 // one (no keys: their rows are written as empty).  Lengths that contradict the
-// buffers are cut to them and reported.
-__device__ __forceinline__ Request load_request(const AttnArgs &a, int b, bool &bad) {
+// buffers are cut to them and reported.  Where offsets descend (BAD_ORDER) requests
+// share tokens, and may be more work than the host's bound of it: the kernels then
+// write every row as empty (write_empty) and take no request.
+__device__ __forceinline__ Request load_request(const AttnArgs &a, int b, uint32_t &bad) {
     Request r;
     const int c0 = a.cu[b], c1 = b < a.B ? a.cu[b + 1] : a.T;
     const int s = b < a.B ? a.seq[b] : 0;
@@ -30,8 +35,16 @@ __device__ __forceinline__ Request load_request(const AttnArgs &a, int b, bool &
     const int e = min(max(c1, r.q0), a.T);
     r.n = e - r.q0;
     r.len = min(max(s, 0), a.max_len);
-    bad |= r.q0 != c0 || e != c1 || r.len != s;
+    bad |= (r.q0 != c0 || e != c1 || r.len != s ? BAD_CUT : 0) | (c1 < c0 && b < a.B ? BAD_ORDER : 0);
     return r;
+}
+
+// All rows of the call as rows without keys, by the whole grid.
+__device__ __forceinline__ void write_empty(const AttnArgs &a) {
+    const int64_t rows = (int64_t)a.T * a.Hq, first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = first; i < rows * (a.D / 8); i += step) reinterpret_cast<uint4 *>(a.out)[i] = make_uint4(0, 0, 0, 0);
+    if (a.lse)
+        for (int64_t i = first; i < rows; i += step) a.lse[i] = -INFINITY;
 }
 
 // Keys [lo, hi) that the rows of tokens [t0, t1) of a request can see.
@@ -73,10 +86,12 @@ __device__ __forceinline__ float soft_cap(float x, const Cap &c) {
     return c.out * (1.0f - __fdividef(2.0f, 1.0f + ex2(u * (2.0f * LOG2E))));
 }
 
-// Inclusive scan of a count a thread over the block, and the total.  U is 32 bits wide
-// wherever the host can bound the total (a 64-bit scan takes twice the shuffles, and a
-// 64-bit division some 400 clocks, each of them on the path of a single token).
-template <int N, class U> __device__ __forceinline__ U block_scan(U mine, U *s_warp, U &total) {
+// Inclusive scan of a count a thread over the block, the total, and whether any thread has
+// `flag` set: then the counts are of no use, and a warp's sum of all ones, which no count
+// comes near, says so (a reducing barrier took 0.3 us more of a single token's 7.2).
+// U is 32 bits wide wherever the host can bound the total (a 64-bit scan takes twice the
+// shuffles, and a 64-bit division some 400 clocks, each of them on the path of a single token).
+template <int N, class U> __device__ __forceinline__ U block_scan(U mine, U *s_warp, U &total, bool &flag) {
     static_assert(N % 32 == 0 && N <= 1024, "whole warps");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     U v = mine;
@@ -85,9 +100,11 @@ template <int N, class U> __device__ __forceinline__ U block_scan(U mine, U *s_w
         const U u = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += u;
     }
+    if (__any_sync(0xffffffffu, flag)) v = ~(U)0;
     if (lane == 31) s_warp[warp] = v;
     __syncthreads();
     U w = lane < N / 32 ? s_warp[lane] : 0;
+    flag = __any_sync(0xffffffffu, w == ~(U)0);
 #pragma unroll
     for (int o = 1; o < N / 32; o <<= 1) {
         const U u = __shfl_up_sync(0xffffffffu, w, o);
@@ -99,7 +116,7 @@ template <int N, class U> __device__ __forceinline__ U block_scan(U mine, U *s_w
 }
 
 // The same for two counts at once.
-template <int N, class U> __device__ __forceinline__ void block_scan2(U &v, U &x, U *s_warp, U &total_v, U &total_x) {
+template <int N, class U> __device__ __forceinline__ void block_scan2(U &v, U &x, U *s_warp, U &total_v, U &total_x, bool &flag) {
     static_assert(N % 32 == 0 && N <= 1024, "whole warps");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
@@ -107,9 +124,11 @@ template <int N, class U> __device__ __forceinline__ void block_scan2(U &v, U &x
         const U a = __shfl_up_sync(0xffffffffu, v, o), b = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) v += a, x += b;
     }
+    if (__any_sync(0xffffffffu, flag)) v = ~(U)0;
     if (lane == 31) s_warp[warp] = v, s_warp[32 + warp] = x;
     __syncthreads();
     U w = lane < N / 32 ? s_warp[lane] : 0, y = lane < N / 32 ? s_warp[32 + lane] : 0;
+    flag = __any_sync(0xffffffffu, w == ~(U)0);
 #pragma unroll
     for (int o = 1; o < N / 32; o <<= 1) {
         const U a = __shfl_up_sync(0xffffffffu, w, o), b = __shfl_up_sync(0xffffffffu, y, o);

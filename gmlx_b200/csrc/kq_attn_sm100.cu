@@ -79,7 +79,8 @@ struct TileArgs {
     uint64_t cap_k[4];
 };
 
-// What the join needs of a pair that block `i` begins and others end; last == i: none.
+// What the join needs of a pair that block `i` begins and others end; last == i: none;
+// last < 0: no request was computed, since offsets descend.
 struct Split {
     int last, q0, n, tok0, h;
 };
@@ -301,7 +302,7 @@ template <int D> struct Walk {
     uint32_t ub, u, ue, before;
     Request rq;
     int b, qt;  // request, pair
-    bool bad;
+    uint32_t bad;
 
     __device__ __forceinline__ static int pair_units(const TileArgs &p, const Request &r, int qt, int &lo, int &hi) {
         const int t0 = qt * NT * p.tile_tok, t1 = min(r.n, t0 + NT * p.tile_tok);
@@ -328,7 +329,7 @@ template <int D> struct Walk {
     }
 
     __device__ __forceinline__ Walk(const TileArgs &p, bool whole, uint32_t ub, uint32_t ue, int b0, uint32_t before0)
-        : p(p), whole(whole), ub(ub), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
+        : p(p), whole(whole), ub(ub), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(0) {
         if (u < ue) rq = load_request(p.a, b, bad);
     }
     __device__ __forceinline__ bool next(Seg &s, uint32_t total, int grid) {
@@ -448,12 +449,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     if (warp == K_WARP && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v) : "memory");
     // units of each thread's run of requests (b == B: the padding tokens)
-    bool bad = false;
+    uint32_t bad = 0;
     const int nb = a.B + 1, per = (nb + THREADS - 1) / THREADS;
     const bool wide = nb <= THREADS / 32;  // few requests: a warp each, a lane a pair
     uint32_t mine = 0, items = 0;
     int most = 0;
-    for (int i = 0; i < per; i++) {
+    for (int i = 0; i < per && !(bad & BAD_ORDER); i++) {  // (up to a descent the tokens are distinct, and their pairs few)
         const int b = wide ? warp : tid * per + i;
         if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad), wide ? lane : 0, wide ? 32 : 1, items, most);
     }
@@ -470,7 +471,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) s_most[warp] = most;
     uint32_t total, pairs, upto = mine, items_upto = items;
-    block_scan2<THREADS, uint32_t>(upto, items_upto, s_warp, total, pairs);
+    bool unordered = bad & BAD_ORDER;
+    block_scan2<THREADS, uint32_t>(upto, items_upto, s_warp, total, pairs, unordered);
+    if (unordered) {  // (the join writes the rows: here that code costs registers, 1.4 of a short prompt's 19 us)
+        if (tid == 0) splits[blockIdx.x].last = -1;
+        tc_before();
+        __syncthreads();
+        tc_after();
+        if (warp == MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(*tmem_slot));
+        return;
+    }
     most = __reduce_max_sync(0xffffffffu, lane < THREADS / 32 ? s_most[lane] : 0);
     const bool whole = pairs <= gridDim.x && most <= (int)((total - PAIR_COST * pairs + gridDim.x - 1) / gridDim.x) + JOIN_COST;
     if (whole) total = pairs, upto = items_upto, mine = items;
@@ -921,6 +931,7 @@ template <bool F16, int D> __global__ void __launch_bounds__(JOIN_T) join_kernel
     const int first = blockIdx.x, sub = threadIdx.x & 15;
     const Split s = reinterpret_cast<const Split *>(a.part)[first];
     if (s.last == first) return;
+    if (s.last < 0) return write_empty(a);
     const int t = blockIdx.y * JOIN_ROWS / TM;
     for (int i = threadIdx.x >> 4; i < JOIN_ROWS; i += JOIN_T / 16) {
         const int row = blockIdx.y * JOIN_ROWS % TM + i, rt = row / a.G, tok = s.tok0 + t * p.tile_tok + rt;

@@ -887,8 +887,9 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     What the cache holds past a request's length, or before every row's window,
     is never used, whatever bytes it has; the values a request does have must be
     finite.  ``max_query_len`` only picks the kernels.  Lengths that contradict
-    the buffers are cut to them (workspace error 20); a page id outside the cache
-    counts as a page of zeros (error 22)."""
+    the buffers are cut to them (workspace error 20), offsets that descend make every
+    row an empty one (error 20); a page id outside the cache counts as a page of
+    zeros (error 22)."""
     if scale is None:
         scale = q.shape[-1] ** -0.5
     e = _ext()

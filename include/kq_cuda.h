@@ -373,7 +373,8 @@ int kq_rope_kv_write(const kq_paged_cache *cache, const void *q, int64_t q_token
  * lse [tokens][heads] f32 (natural log of the row's sum) or NULL.  Rows without
  * keys, and tokens past cu_seqlens[batch], give 0 and -inf.  dim is 64, 128 or
  * 256; heads a multiple of kv_heads.  max_query_len only picks the kernels: a
- * longer request is still computed in full. */
+ * longer request is still computed in full.  Where cu_seqlens descends, no
+ * request is computed: every row is written as one without keys (error 20). */
 int kq_paged_attention(const kq_paged_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
                        int64_t tokens, int64_t heads, const int32_t *block_tables, int64_t table_stride,
                        int64_t table_width, const int32_t *seq_lens, const int32_t *cu_seqlens, int64_t batch,

@@ -5,7 +5,7 @@ import torch
 
 from gmlx_b200 import kq
 
-from test_gpu_serve_ops import BF, FP, attn_inputs, check_attn
+from test_gpu_serve_ops import BF, FP, INF, attn_inputs, check_attn, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -50,3 +50,26 @@ def test_expanded_heads_are_turned_and_stored(cuda):
         kc, vc = torch.zeros(2, 2, 4, 2, 64, device=cuda, dtype=BF)
         outs.append((kq.rope_kv_write(*args, angle.cos(), angle.sin(), slots.int(), kc, vc, slots), kc, vc))
     assert all(torch.equal(a, b) for a, b in zip(*outs)) and kq.workspace_error() == 0
+
+
+@pytest.mark.parametrize("max_q", [1, 1000])
+@pytest.mark.parametrize("b,t,hq,hk,d,keys", [(1000, 1000, 32, 8, 128, 1024), (64, 8192, 32, 8, 64, 16384), (2, 7, 4, 2, 256, 64),
+                                              (1500, 300, 8, 8, 64, 300)])
+def test_descending_offsets_leave_every_row_empty(cuda, b, t, hq, hk, d, keys, max_q):
+    """Requests that share tokens are far more work than the tokens there are: no request
+    is computed, nothing is left behind in the workspace, and later calls are right."""
+    valid = attn_inputs(cuda, [(1, 5000), (1, 40), (70, 900)], 8, 2, d, 16, BF)
+    good = kq.paged_attention(*valid, 70, return_lse=True)
+    q = torch.randn(t, hq, d, device=cuda).to(BF)
+    kc, vc = torch.randn(2, 4, 64, hk, d, device=cuda).to(BF)
+    table = torch.zeros(b, -(-keys // 64), dtype=torch.int32, device=cuda)
+    for cu in ([0 if i % 2 == 0 else t for i in range(b + 1)], [0] + [t] * (b - 1) + [t - 1]):
+        out, lse = kq.paged_attention(q, kc, vc, table, i32([keys] * b, cuda), i32(cu, cuda), max_q, return_lse=True)
+        assert kq.workspace_error() == 20 and kq.workspace_error() == 0
+        assert (out == 0).all() and (lse == -INF).all()
+        key = (torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
+        ws = kq._ext().workspace_peek(*key) if kq._ext() is not None else kq._WS[key]
+        assert not ws[:256 + (1 << 20)].any()  # error word and counters
+        again = kq.paged_attention(*valid, 70, return_lse=True)
+        assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1])
+    assert kq.workspace_error() == 0
