@@ -305,12 +305,12 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
         float *part = a.part + (int64_t)(blockIdx.x * 2 + (k0 == 0 ? 1 : 0)) * part_floats(D);
         auto store = [&](int row, int d, float4 v, float mr, float lr) {
             const int r = rt * ROWS + row;
-            const float inv = lr > 0.f ? 1.0f / lr : 0.f;
+            const float inv = lr == 0.f ? 0.f : 1.0f / lr;  // (0: no key; a NaN stays one)
             const int tok = row_token(a, r);
             const int64_t orow = (int64_t)(rq.q0 + tok) * a.Hq + h * a.G + r - tok * a.G;
             uint2 w = make_uint2(pack_half<F16>(v.x * inv, v.y * inv), pack_half<F16>(v.z * inv, v.w * inv));
             *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + d) = w;
-            if (d == 0 && a.lse) a.lse[orow] = lr > 0.f ? mr * LN2 + logf(lr) : -INFINITY;
+            if (d == 0 && a.lse) a.lse[orow] = lr == 0.f ? -INFINITY : mr * LN2 + logf(lr);
         };
         for (int idx = tid; idx < nrows * (D / 4); idx += NW * 32) {
             const int row = idx / (D / 4), d = idx % (D / 4) * 4;

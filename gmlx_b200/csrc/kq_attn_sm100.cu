@@ -872,12 +872,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int row = row0 + 8 * r;
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
                 l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                inv[r] = l[r] > 0.f ? 1.0f / l[r] : 0.f;
+                inv[r] = l[r] == 0.f ? 0.f : 1.0f / l[r];  // (0: no key; a NaN stays one)
                 orow[r] = (int64_t)(s.q0 + tok0 + (r ? rt1 : rt0)) * a.Hq + s.h * a.G + row - (r ? rt1 : rt0) * a.G;
                 const float ml = ref[r] * sl2;  // log2 units
                 if (q2 == 0) {
-                    if (split) part[row] = l[r] > 0.f ? ml : -INFINITY, part[TM + row] = l[r];
-                    else if (live[r] && a.lse) a.lse[orow[r]] = l[r] > 0.f ? ml * LN2 + logf(l[r]) : -INFINITY;
+                    if (split) part[row] = l[r] == 0.f ? -INFINITY : ml, part[TM + row] = l[r];
+                    else if (live[r] && a.lse) a.lse[orow[r]] = l[r] == 0.f ? -INFINITY : ml * LN2 + logf(l[r]);
                 }
             }
             if (split && c == 0) continue;
@@ -953,13 +953,13 @@ template <bool F16, int D> __global__ void __launch_bounds__(JOIN_T) join_kernel
                 if (w != 0.f) acc[k].x += w * v.x, acc[k].y += w * v.y, acc[k].z += w * v.z, acc[k].w += w * v.w;
             }
         }
-        const float inv = l > 0.f ? 1.0f / l : 0.f;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
         const int64_t orow = (int64_t)(s.q0 + tok) * a.Hq + s.h * a.G + row - rt * a.G;
 #pragma unroll
         for (int k = 0; k < D / 64; k++)
             *reinterpret_cast<uint2 *>(reinterpret_cast<uint16_t *>(a.out) + orow * D + (sub + k * 16) * 4) =
                 make_uint2(pack_half<F16>(acc[k].x * inv, acc[k].y * inv), pack_half<F16>(acc[k].z * inv, acc[k].w * inv));
-        if (sub == 0 && a.lse) a.lse[orow] = l > 0.f ? m * LN2 + logf(l) : -INFINITY;
+        if (sub == 0 && a.lse) a.lse[orow] = l == 0.f ? -INFINITY : m * LN2 + logf(l);
     }
 }
 

@@ -886,7 +886,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     A row that sees no key, and tokens past the last request, give 0 and -inf.
     What the cache holds past a request's length, or before every row's window,
     is never used, whatever bytes it has; the values a request does have must be
-    finite.  ``max_query_len`` only picks the kernels.  Lengths that contradict
+    finite, and a NaN query or key makes NaN of the rows that see it.  ``max_query_len`` only picks the kernels.  Lengths that contradict
     the buffers are cut to them (workspace error 20), offsets that descend make every
     row an empty one (error 20); a page id outside the cache counts as a page of
     zeros (error 22)."""

@@ -5,7 +5,7 @@ import torch
 
 from gmlx_b200 import kq
 
-from test_gpu_serve_ops import BF, FP, INF, attn_inputs, check_attn, i32
+from test_gpu_serve_ops import BF, FP, INF, attn_inputs, attn_ref, check_attn, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -72,4 +72,24 @@ def test_descending_offsets_leave_every_row_empty(cuda, b, t, hq, hk, d, keys, m
         assert not ws[:256 + (1 << 20)].any()  # error word and counters
         again = kq.paged_attention(*valid, 70, return_lse=True)
         assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1])
+    assert kq.workspace_error() == 0
+
+
+@pytest.mark.parametrize("d,dtype", [(64, FP), (128, BF), (256, BF)])
+@pytest.mark.parametrize("lens", [[(1, 5000), (1, 30)], [(150, 5000), (40, 40)]])
+def test_nan_reaches_its_rows_and_no_others(cuda, lens, d, dtype):
+    """A NaN query, and a NaN key in the last position of a request (one row sees it):
+    those rows are NaN, sum and output, however the row is split; the others are as without."""
+    args = attn_inputs(cuda, lens, 4, 2, d, 16, dtype)
+    ref, ref_l, tol, tol_l = attn_ref(*args, d ** -0.5, 0, 0.0, True)
+    q, kc = args[0].clone(), args[1].clone()
+    q[0, 1, 3] = float("nan")
+    last = lens[0][1] - 1
+    kc[args[3][0, last // 16].long(), last % 16, 1, 5] = float("nan")  # kv head 1: query heads 2 and 3
+    out, lse = kq.paged_attention(q, kc, *args[2:], max(n for n, _ in lens), return_lse=True)
+    hit = torch.zeros(lse.shape, dtype=torch.bool, device=cuda)
+    hit[0, 1] = True
+    hit[lens[0][0] - 1, 2:] = True
+    assert lse[hit].isnan().all() and out[hit].isnan().all()
+    assert ((out.double() - ref).abs() <= tol)[~hit].all() and ((lse.double() - ref_l).abs() <= tol_l)[~hit].all()
     assert kq.workspace_error() == 0
