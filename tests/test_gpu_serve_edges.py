@@ -69,7 +69,7 @@ def test_descending_offsets_leave_every_row_empty(cuda, b, t, hq, hk, d, keys, m
         assert (out == 0).all() and (lse == -INF).all()
         key = (torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
         ws = kq._ext().workspace_peek(*key) if kq._ext() is not None else kq._WS[key]
-        assert not ws[:256 + (1 << 20)].any()  # error word and counters
+        assert not ws[256:256 + (1 << 20)].any()  # the counters (in front, the group count of an expert call may stand)
         again = kq.paged_attention(*valid, 70, return_lse=True)
         assert torch.equal(again[0], good[0]) and torch.equal(again[1], good[1])
     assert kq.workspace_error() == 0
