@@ -25,6 +25,7 @@
 #include <map>
 #include <mutex>
 #include <tuple>
+#include <vector>
 
 #include "../../include/kq_cuda.h"
 
@@ -41,7 +42,12 @@ GluFn g_glu = nullptr;
 WsFn g_matmul_ws = nullptr, g_glu_ws = nullptr;
 
 std::mutex g_mu;
-std::map<std::pair<int, int64_t>, at::Tensor> g_ws;                    // (device, stream) -> workspace
+struct Workspace {
+    at::Tensor now;
+    bool captured = false;         // a graph was captured with `now`
+    std::vector<at::Tensor> kept;  // workspaces outgrown since that graphs were captured with
+};
+std::map<std::pair<int, int64_t>, Workspace> g_ws;                     // (device, stream) -> workspace
 std::map<std::tuple<int, int, int64_t, int64_t, int64_t>, size_t> g_ws_bytes;  // (op, codec, m, n, k) -> bytes
 
 int dtype_code(at::ScalarType t) {
@@ -56,24 +62,46 @@ void set_entry_points(int64_t matmul, int64_t glu, int64_t matmul_ws, int64_t gl
 }
 
 // The zero-filled workspace of (device, stream), grown to at least nbytes
-// (at least 1 MiB); the library leaves every workspace zero after each call.
+// (at least 1 MiB); the library leaves every workspace zero after each call but
+// for the error word in front, which goes along when it grows.  A workspace that
+// a graph was captured with stays for the graph's replays.
 at::Tensor workspace(int64_t device, int64_t stream, int64_t nbytes) {
     std::lock_guard<std::mutex> lk(g_mu);
     auto key = std::make_pair((int)device, stream);
-    auto it = g_ws.find(key);
-    if (it != g_ws.end() && it->second.numel() >= nbytes) return it->second;
-    if (nbytes <= 0 && it != g_ws.end()) return it->second;
-    const int64_t sz = nbytes > (1 << 20) ? nbytes : (1 << 20);
-    at::Tensor t = at::zeros({sz}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (int)device));
-    g_ws[key] = t;
-    return t;
+    Workspace &w = g_ws[key];
+    if (!w.now.defined() || w.now.numel() < nbytes) {
+        const int64_t sz = nbytes > (1 << 20) ? nbytes : (1 << 20);
+        at::Tensor t = at::zeros({sz}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (int)device));
+        if (w.now.defined()) {
+            t.narrow(0, 0, 4).copy_(w.now.narrow(0, 0, 4), true);
+            if (w.captured) w.kept.push_back(w.now);
+        }
+        w.now = t, w.captured = false;
+    }
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (!w.captured) {
+        if (cudaStreamIsCapturing(reinterpret_cast<cudaStream_t>(stream), &cap) == cudaSuccess) w.captured = cap != cudaStreamCaptureStatusNone;
+        else (void)cudaGetLastError();  // the default stream beside a capture: the call itself will say so
+    }
+    return w.now;
 }
 
 // The existing workspace of (device, stream), or an undefined tensor.
 at::Tensor workspace_peek(int64_t device, int64_t stream) {
     std::lock_guard<std::mutex> lk(g_mu);
     auto it = g_ws.find(std::make_pair((int)device, stream));
-    return it == g_ws.end() ? at::Tensor() : it->second;
+    return it == g_ws.end() ? at::Tensor() : it->second.now;
+}
+
+// All workspaces of (device, stream) that a call or a graph may still write to.
+std::vector<at::Tensor> workspaces(int64_t device, int64_t stream) {
+    std::lock_guard<std::mutex> lk(g_mu);
+    std::vector<at::Tensor> all;
+    auto it = g_ws.find(std::make_pair((int)device, stream));
+    if (it == g_ws.end()) return all;
+    if (it->second.now.defined()) all.push_back(it->second.now);
+    all.insert(all.end(), it->second.kept.begin(), it->second.kept.end());
+    return all;
 }
 
 size_t ws_bytes(int op, int codec, int64_t m, int64_t n, int64_t k) {
@@ -316,6 +344,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("set_entry_points", &set_entry_points);
     m.def("workspace", &workspace);
     m.def("workspace_peek", &workspace_peek);
+    m.def("workspaces", &workspaces);
     m.def("quantized_matmul", &quantized_matmul);
     m.def("quantized_glu", &quantized_glu);
     m.def("set_serve_entry_points", &set_serve_entry_points);

@@ -149,8 +149,11 @@ def _rows2d(w: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 # --------------------------------------------------------------------------
 # per-(device, stream) workspaces, zero-filled once and kept zero by the library
+# (the error word in front goes along when one grows)
 
 _WS: dict[tuple[int, int], torch.Tensor] = {}
+_WS_CAPTURED: set[tuple[int, int]] = set()  # a graph was captured with the workspace
+_WS_KEPT: dict[tuple[int, int], list[torch.Tensor]] = {}  # outgrown ones that graphs still write to
 
 
 _WS_SIZE: dict[tuple, int] = {}
@@ -207,20 +210,27 @@ def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
         return e.workspace(key[0], key[1], nbytes)
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
+        old, ws = ws, torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
+        if old is not None:
+            ws[:4].copy_(old[:4], non_blocking=True)
+            if key in _WS_CAPTURED:
+                _WS_KEPT.setdefault(key, []).append(old)
+                _WS_CAPTURED.discard(key)
         _WS[key] = ws
+    if torch.cuda.is_current_stream_capturing():
+        _WS_CAPTURED.add(key)
     return ws
 
 
 def workspace_error(device=None, clear: bool = True) -> int:
-    """Device-side error word of the current stream's workspace (syncs)."""
+    """Device-side error word of the current stream's workspace (syncs); workspaces
+    that were outgrown but still serve a captured graph are looked at too."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     key = (dev.index, torch.cuda.current_stream(dev).cuda_stream)
     e = _ext()
-    ws = e.workspace_peek(key[0], key[1]) if e is not None else _WS.get(key)
-    if ws is None:  # (an undefined tensor from the extension arrives as None)
-        return 0
-    return _lib.load().kq_workspace_error(_p(ws), int(clear), _stream(dev))
+    all_ws = e.workspaces(key[0], key[1]) if e is not None else [w for w in [_WS.get(key)] if w is not None] + _WS_KEPT.get(key, [])
+    codes = [_lib.load().kq_workspace_error(_p(ws), int(clear), _stream(dev)) for ws in all_ws]
+    return next((c for c in codes if c), 0)
 
 
 # --------------------------------------------------------------------------

@@ -5,7 +5,7 @@ import torch
 
 from gmlx_b200 import kq
 
-from test_gpu_serve_ops import BF, FP, INF, attn_inputs, attn_ref, check_attn, i32
+from test_gpu_serve_ops import BF, FP, INF, attn_inputs, attn_ref, check_attn, i32, slow
 
 pytestmark = pytest.mark.gpu
 
@@ -93,3 +93,67 @@ def test_nan_reaches_its_rows_and_no_others(cuda, lens, d, dtype):
     assert lse[hit].isnan().all() and out[hit].isnan().all()
     assert ((out.double() - ref).abs() <= tol)[~hit].all() and ((lse.double() - ref_l).abs() <= tol_l)[~hit].all()
     assert kq.workspace_error() == 0
+
+
+def fresh_stream(cuda):
+    """A stream that no call has used (handles of destroyed streams may come again)."""
+    for _ in range(64):
+        s = torch.cuda.Stream()
+        key = (torch.cuda.current_device(), s.cuda_stream)
+        e = kq._ext()
+        if (e.workspace_peek(*key) is None if e is not None else True) and key not in kq._WS:
+            return s
+    pytest.skip("no unused stream")
+
+
+def overdrawn_plan(cuda):
+    kq.paged_plan(i32([0], cuda), i32([4], cuda), i32([[-1]], cuda), i32([], cuda), 4, 4)
+
+
+@pytest.mark.parametrize("call", [lambda f, *a: f(*a), slow], ids=["native", "python"])
+def test_a_growing_workspace_keeps_its_error_word(cuda, call):
+    """The plan's missing page is still reported after the stream's first attention."""
+    args = attn_inputs(cuda, [(2, 30)], 4, 2, 64, 16, BF)
+    s = fresh_stream(cuda)
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call(overdrawn_plan, cuda)
+        call(kq.paged_attention, *args, 2)
+        assert call(kq.workspace_error) == 21 and call(kq.workspace_error) == 0
+
+
+@pytest.mark.parametrize("call", [lambda f, *a: f(*a), slow], ids=["native", "python"])
+def test_a_captured_workspace_outlives_its_growth(cuda, call):
+    """A graph keeps the workspace it was captured with, to itself, and errors that its
+    replays record there are seen."""
+    small = attn_inputs(cuda, [(1, 900)], 4, 2, 64, 16, BF)
+    large = attn_inputs(cuda, [(1, 900)], 4, 2, 256, 16, BF)
+    seq = small[4].clone()
+    s = fresh_stream(cuda)
+    s.wait_stream(torch.cuda.current_stream())
+    key = (torch.cuda.current_device(), s.cuda_stream)
+
+    def workspace():
+        return kq._ext().workspace_peek(*key) if kq._EXT else kq._WS[key]
+
+    with torch.cuda.stream(s):
+        ref = call(kq.paged_attention, *small, 1)
+    s.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=s):
+        out = call(kq.paged_attention, *small[:4], seq, small[5], 1)
+    with torch.cuda.stream(s):
+        old = call(workspace)
+        lo, size = old.data_ptr(), old.numel()
+        del old
+        call(kq.paged_attention, *large, 1)
+        assert call(workspace).data_ptr() != lo
+        # what the caching allocator hands out now must not be the graph's workspace
+        others = [torch.full((size,), 255, dtype=torch.uint8, device=cuda) for _ in range(4)]
+        assert all(t.data_ptr() + size <= lo or lo + size <= t.data_ptr() for t in others)
+        g.replay()
+        assert torch.equal(out, ref) and all((t == 255).all() for t in others)
+        assert call(kq.workspace_error) == 0
+        seq.fill_(10 ** 6)
+        g.replay()
+        assert call(kq.workspace_error) == 20 and call(kq.workspace_error) == 0
