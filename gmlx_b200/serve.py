@@ -64,7 +64,10 @@ class PagedKVCache:
         need = sum(self._pages(t) - self._pages(c) for t, c in zip(total, self.lens))
         if need > self.free.shape[0]:
             raise ValueError(f"plan: {need} pages needed, {self.free.shape[0]} free")
-        ctx, new = torch.tensor([self.lens, list(query_lens)], dtype=torch.int32).to(self.free.device)
+        # (from pinned memory, which the allocator holds until the copy is done: from other
+        # memory the copy would wait for all that is queued)
+        ctx, new = torch.tensor([self.lens, list(query_lens)], dtype=torch.int32,
+                                pin_memory=self.free.is_cuda).to(self.free.device, non_blocking=True)
         p = kq.paged_plan(ctx, new, self.tables, self.free, self.page_size, sum(query_lens))
         self.free, self.lens = self.free[need:], total
         return Step(p, max(query_lens, default=0))

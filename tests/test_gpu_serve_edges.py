@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from gmlx_b200 import kq
+from gmlx_b200 import kq, serve
 
 from test_gpu_serve_ops import BF, FP, INF, attn_inputs, attn_ref, check_attn, i32, slow
 
@@ -157,3 +157,35 @@ def test_a_captured_workspace_outlives_its_growth(cuda, call):
         seq.fill_(10 ** 6)
         g.replay()
         assert call(kq.workspace_error) == 20 and call(kq.workspace_error) == 0
+
+
+def test_a_step_does_not_wait_for_the_device(cuda):
+    layer = serve.PagedDecoderLayer(512, 8, 2, 64, 8, 2, 256, device=cuda)
+    cache = serve.PagedKVCache(1, 16, 16, 2, 64, 2, device=cuda)
+    cos, sin = serve.rope_tables(256, 64, device=cuda)
+    x = torch.zeros(6, 512, device=cuda, dtype=BF)
+    layer(x, cos, sin, cache, 0, cache.plan([5, 1]))  # kernels are loaded, workspaces made
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        step = cache.plan([1, 5])
+        layer(x, cos, sin, cache, 0, step)
+        cache.release(0)
+        cache.plan([3, 0])
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert step.plan.seq_lens.tolist() == [6, 6] and kq.workspace_error() == 0
+
+
+def test_lengths_of_many_steps_in_flight(cuda):
+    """Plans that are queued faster than the device takes them: each sees its own lengths."""
+    cache = serve.PagedKVCache(1, 64, 16, 1, 64, 3, device=cuda)
+    a = torch.randn(4096, 4096, device=cuda)
+    torch.cuda.synchronize()
+    for _ in range(20):  # the device is busy for some milliseconds
+        a = a @ a * 1e-2
+    steps = [cache.plan([i % 3, 1, 0]) for i in range(100)]
+    lens = [0, 0, 0]
+    for i, s in enumerate(steps):
+        lens = [lens[0] + i % 3, lens[1] + 1, 0]
+        assert s.plan.seq_lens.tolist() == lens
+    assert kq.workspace_error() == 0
