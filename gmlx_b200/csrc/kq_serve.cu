@@ -246,9 +246,12 @@ __global__ void __launch_bounds__(ROPE_T) rope_kernel(const RopeArgs a) {
 // 13.3 us; 64 tokens 4.9 us, one token of 128 experts 2.8 us, of which the launch
 // is 2.3 and the chain load, scores, k rounds the rest.
 
-__device__ __forceinline__ uint32_t ordered(float f) {  // NaN below everything
+// Experts of closed groups come behind those of open ones, also behind what a bias of -inf
+// rules out there (0: no expert, or one that is chosen already).
+constexpr uint32_t CLOSED = 1u;
+__device__ __forceinline__ uint32_t ordered(float f) {  // NaN below every number
     const uint32_t b = __float_as_uint(f + 0.0f);
-    if (f != f) return 1u;
+    if (f != f) return CLOSED + 1u;
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(ROUTE_W * 32, PER <= 8 ? 16 : 1) route_kernel(
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int e = lane + 32 * i;
-            key[i] = e >= a.E ? 0u : (kept >> ((shift >= 0 ? e >> shift : e / size) * lg)) & 1u ? ordered(kb[e]) : ordered(-INFINITY);
+            key[i] = e >= a.E ? 0u : (kept >> ((shift >= 0 ? e >> shift : e / size) * lg)) & 1u ? ordered(kb[e]) : CLOSED;
         }
     } else {
 #pragma unroll

@@ -189,3 +189,21 @@ def test_lengths_of_many_steps_in_flight(cuda):
         lens = [lens[0] + i % 3, lens[1] + 1, 0]
         assert s.plan.seq_lens.tolist() == lens
     assert kq.workspace_error() == 0
+
+
+@pytest.mark.parametrize("e,groups", [(64, 8), (512, 4)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_stays_in_the_open_groups(cuda, e, groups, scoring):
+    """Experts that the bias rules out (-inf), so that fewer than k are left in the open
+    groups: the rest of the choice are the ruled-out ones there, lowest first."""
+    size, k = e // groups, 8
+    first = e - 2 * size
+    logits = torch.randn(33, e, device=cuda)
+    bias = torch.full((e,), -10.0, device=cuda)
+    bias[first:] = -INF
+    left = [first + 2, first + 3, e - 3, e - 2]  # two of each of the last two groups, which rank highest
+    bias[left] = 0.0
+    idx, w = kq.moe_route(logits, k, scoring, bias, groups, 2)
+    rest = [i for i in range(first, e) if i not in left][:k - 4]
+    assert all(set(r[:4]) == set(left) and r[4:] == rest for r in idx.tolist())
+    assert torch.isfinite(w).all()
