@@ -73,8 +73,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
     __shared__ int s_b, s_last;
     __shared__ Request s_rq;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    uint32_t bad = 0;
-    bool bad_page = false;
+    bool bad = false, bad_page = false, unordered = false;
 
     // units of each thread's run of requests (b == B: the padding tokens)
     const int nb = a.B + 1, per = (nb + NW * 32 - 1) / (NW * 32);
@@ -82,10 +81,9 @@ __global__ void __launch_bounds__(NW * 32, CTAS) rows_kernel(const __grid_consta
     Request rq;
     for (int i = 0; i < per; i++) {
         const int b = tid * per + i;
-        if (b < nb) mine += request_units<U>(a, rq = load_request(a, b, bad));
+        if (b < nb) mine += request_units<U>(a, rq = load_request(a, b, bad)), unordered |= descends(a, b);
     }
     U total;
-    bool unordered = bad & BAD_ORDER;
     const U upto = block_scan<NW * 32, U>(mine, s_warp, total, unordered);
     if (blockIdx.x == 0 && bad) atomicCAS(a.err, 0, ERR_LENGTHS);
     if (unordered) return write_empty(a);

@@ -19,15 +19,12 @@ struct Request {
     int q0, n, len;
 };
 
-// What load_request finds wrong: lengths or offsets cut to the buffers; offsets that descend.
-constexpr uint32_t BAD_CUT = 1, BAD_ORDER = 2;
-
 // Request b of the call; b == B stands for the padding tokens behind the last
 // one (no keys: their rows are written as empty).  Lengths that contradict the
-// buffers are cut to them and reported.  Where offsets descend (BAD_ORDER) requests
-// share tokens, and may be more work than the host's bound of it: the kernels then
-// write every row as empty (write_empty) and take no request.
-__device__ __forceinline__ Request load_request(const AttnArgs &a, int b, uint32_t &bad) {
+// buffers are cut to them and reported.  Where offsets descend (descends) requests share
+// tokens, and may be more work than the host's bound of it: the kernels then write every
+// row as empty (write_empty) and take no request.
+__device__ __forceinline__ Request load_request(const AttnArgs &a, int b, bool &bad) {
     Request r;
     const int c0 = a.cu[b], c1 = b < a.B ? a.cu[b + 1] : a.T;
     const int s = b < a.B ? a.seq[b] : 0;
@@ -35,9 +32,10 @@ __device__ __forceinline__ Request load_request(const AttnArgs &a, int b, uint32
     const int e = min(max(c1, r.q0), a.T);
     r.n = e - r.q0;
     r.len = min(max(s, 0), a.max_len);
-    bad |= (r.q0 != c0 || e != c1 || r.len != s ? BAD_CUT : 0) | (c1 < c0 && b < a.B ? BAD_ORDER : 0);
+    bad |= r.q0 != c0 || e != c1 || r.len != s;
     return r;
 }
+__device__ __forceinline__ bool descends(const AttnArgs &a, int b) { return b < a.B && a.cu[b + 1] < a.cu[b]; }
 
 // All rows of the call as rows without keys, by the whole grid.
 __device__ __forceinline__ void write_empty(const AttnArgs &a) {

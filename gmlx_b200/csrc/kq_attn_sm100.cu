@@ -302,7 +302,7 @@ template <int D> struct Walk {
     uint32_t ub, u, ue, before;
     Request rq;
     int b, qt;  // request, pair
-    uint32_t bad;
+    bool bad;
 
     __device__ __forceinline__ static int pair_units(const TileArgs &p, const Request &r, int qt, int &lo, int &hi) {
         const int t0 = qt * NT * p.tile_tok, t1 = min(r.n, t0 + NT * p.tile_tok);
@@ -329,7 +329,7 @@ template <int D> struct Walk {
     }
 
     __device__ __forceinline__ Walk(const TileArgs &p, bool whole, uint32_t ub, uint32_t ue, int b0, uint32_t before0)
-        : p(p), whole(whole), ub(ub), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(0) {
+        : p(p), whole(whole), ub(ub), u(ub), ue(ue), before(before0), b(b0), qt(0), bad(false) {
         if (u < ue) rq = load_request(p.a, b, bad);
     }
     __device__ __forceinline__ bool next(Seg &s, uint32_t total, int grid) {
@@ -449,14 +449,14 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     if (warp == K_WARP && lane < 3) asm volatile("prefetch.tensormap [%0];" ::"l"(lane == 0 ? &tm_q : lane == 1 ? &tm_k : &tm_v) : "memory");
     // units of each thread's run of requests (b == B: the padding tokens)
-    uint32_t bad = 0;
+    bool bad = false, unordered = false;
     const int nb = a.B + 1, per = (nb + THREADS - 1) / THREADS;
     const bool wide = nb <= THREADS / 32;  // few requests: a warp each, a lane a pair
     uint32_t mine = 0, items = 0;
     int most = 0;
-    for (int i = 0; i < per && !(bad & BAD_ORDER); i++) {  // (up to a descent the tokens are distinct, and their pairs few)
+    for (int i = 0; i < per && !unordered; i++) {  // (up to a descent the tokens are distinct, and their pairs few)
         const int b = wide ? warp : tid * per + i;
-        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad), wide ? lane : 0, wide ? 32 : 1, items, most);
+        if (b < nb) mine += Walk<D>::request_units(p, load_request(a, b, bad), wide ? lane : 0, wide ? 32 : 1, items, most), unordered = descends(a, b);
     }
     if (wide) {
         mine = __reduce_add_sync(0xffffffffu, mine), items = __reduce_add_sync(0xffffffffu, items);
@@ -471,7 +471,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     most = __reduce_max_sync(0xffffffffu, most);
     if (lane == 0) s_most[warp] = most;
     uint32_t total, pairs, upto = mine, items_upto = items;
-    bool unordered = bad & BAD_ORDER;
     block_scan2<THREADS, uint32_t>(upto, items_upto, s_warp, total, pairs, unordered);
     if (unordered) {  // (the join writes the rows: here that code costs registers, 1.4 of a short prompt's 19 us)
         if (tid == 0) splits[blockIdx.x].last = -1;
