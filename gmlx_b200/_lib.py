@@ -80,6 +80,7 @@ SIGNATURES = {
     "kq_ipc_handle": (_i32, [_vp, _vp]),
     "kq_ipc_open": (_i32, [_vp, _vp]),
     "kq_ipc_close": (_i32, [_vp]),
+    "kq_capture_mode": (_i32, [_i32]),
     "kq_paged_plan": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _sz,
                              _vp]),
     "kq_rope_kv_write": (_i32, [_vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _i64, _i32,

@@ -1062,6 +1062,11 @@ int kq_quantized_matmul_chain(const kq_chain_problem *problems, int count, int x
     return KQ_OK;
 }
 
+int kq_capture_mode(int mode) {
+    cudaStreamCaptureMode m = (cudaStreamCaptureMode)mode;
+    return mode < 0 || mode > 2 || cudaThreadExchangeStreamCaptureMode(&m) != cudaSuccess ? -1 : (int)m;
+}
+
 int kq_workspace_error(void *workspace, int clear, void *stream) {
     if (!workspace) return 0;
     int v = 0;

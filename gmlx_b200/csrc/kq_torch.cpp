@@ -18,6 +18,7 @@
 // uses too (workspace()), so kq.workspace_error() sees every call's error word.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -45,7 +46,7 @@ std::mutex g_mu;
 struct Workspace {
     at::Tensor now;
     bool captured = false;         // a graph was captured with `now`
-    std::vector<at::Tensor> kept;  // workspaces outgrown since that graphs were captured with
+    std::vector<at::Tensor> kept;  // workspaces outgrown since that graphs write to, or that a capture outgrew
 };
 std::map<std::pair<int, int64_t>, Workspace> g_ws;                     // (device, stream) -> workspace
 std::map<std::tuple<int, int, int64_t, int64_t, int64_t>, size_t> g_ws_bytes;  // (op, codec, m, n, k) -> bytes
@@ -61,6 +62,27 @@ void set_entry_points(int64_t matmul, int64_t glu, int64_t matmul_ws, int64_t gl
     g_glu_ws = reinterpret_cast<WsFn>(glu_ws);
 }
 
+bool capturing(cudaStream_t s) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &cap) == cudaSuccess) return cap != cudaStreamCaptureStatusNone;
+    (void)cudaGetLastError();  // the default stream beside a capture: the call itself will say so
+    return false;
+}
+
+// A new workspace.  Made in a capture it is allocated and zeroed outside of it, or every
+// replay would zero it again.
+at::Tensor zeroed(int device, int64_t sz, bool in_capture) {
+    const auto opt = at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device);
+    if (!in_capture) return at::zeros({sz}, opt);
+    c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+    c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)device);
+    for (int i = 0; i < 64 && capturing(side.stream()); i++) side = c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)device);
+    c10::cuda::CUDAStreamGuard guard(side);
+    at::Tensor t = at::zeros({sz}, opt);
+    side.synchronize();
+    return t;
+}
+
 // The zero-filled workspace of (device, stream), grown to at least nbytes
 // (at least 1 MiB); the library leaves every workspace zero after each call but
 // for the error word in front, which goes along when it grows.  A workspace that
@@ -71,18 +93,15 @@ at::Tensor workspace(int64_t device, int64_t stream, int64_t nbytes) {
     Workspace &w = g_ws[key];
     if (!w.now.defined() || w.now.numel() < nbytes) {
         const int64_t sz = nbytes > (1 << 20) ? nbytes : (1 << 20);
-        at::Tensor t = at::zeros({sz}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (int)device));
+        const bool in_capture = capturing(reinterpret_cast<cudaStream_t>(stream));
+        at::Tensor t = zeroed((int)device, sz, in_capture);
         if (w.now.defined()) {
-            t.narrow(0, 0, 4).copy_(w.now.narrow(0, 0, 4), true);
-            if (w.captured) w.kept.push_back(w.now);
+            if (!in_capture) t.narrow(0, 0, 4).copy_(w.now.narrow(0, 0, 4), true);
+            if (in_capture || w.captured) w.kept.push_back(w.now);
         }
-        w.now = t, w.captured = false;
-    }
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    if (!w.captured) {
-        if (cudaStreamIsCapturing(reinterpret_cast<cudaStream_t>(stream), &cap) == cudaSuccess) w.captured = cap != cudaStreamCaptureStatusNone;
-        else (void)cudaGetLastError();  // the default stream beside a capture: the call itself will say so
-    }
+        w.now = t, w.captured = in_capture;
+    } else if (!w.captured)
+        w.captured = capturing(reinterpret_cast<cudaStream_t>(stream));
     return w.now;
 }
 

@@ -153,7 +153,7 @@ def _rows2d(w: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 _WS: dict[tuple[int, int], torch.Tensor] = {}
 _WS_CAPTURED: set[tuple[int, int]] = set()  # a graph was captured with the workspace
-_WS_KEPT: dict[tuple[int, int], list[torch.Tensor]] = {}  # outgrown ones that graphs still write to
+_WS_KEPT: dict[tuple[int, int], list[torch.Tensor]] = {}  # outgrown ones that graphs write to, or that a capture outgrew
 
 
 _WS_SIZE: dict[tuple, int] = {}
@@ -202,6 +202,26 @@ def _fast_codec(codec):
     return v
 
 
+def _zeroed(dev: torch.device, nbytes: int, in_capture: bool) -> torch.Tensor:
+    """A new workspace; made in a capture it is allocated and zeroed outside of it, or
+    every replay would zero it again."""
+    if not in_capture:
+        return torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+    mode = _lib.load().kq_capture_mode(2)
+    try:
+        for _ in range(64):
+            side = torch.cuda.Stream(dev)
+            with torch.cuda.stream(side):
+                if torch.cuda.is_current_stream_capturing():
+                    continue  # (the pool hands its streams out in turn)
+                ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+            side.synchronize()
+            return ws
+    finally:
+        _lib.load().kq_capture_mode(mode)
+    raise RuntimeError("no stream to zero a workspace on during a capture")
+
+
 def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
     key = (dev.index if dev.index is not None else torch.cuda.current_device(),
            torch.cuda.current_stream(dev).cuda_stream)
@@ -210,10 +230,12 @@ def _workspace(dev: torch.device, nbytes: int) -> torch.Tensor:
         return e.workspace(key[0], key[1], nbytes)
     ws = _WS.get(key)
     if ws is None or ws.numel() < nbytes:
-        old, ws = ws, torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=dev)
+        in_capture = torch.cuda.is_current_stream_capturing()
+        old, ws = ws, _zeroed(dev, max(nbytes, 1 << 20), in_capture)
         if old is not None:
-            ws[:4].copy_(old[:4], non_blocking=True)
-            if key in _WS_CAPTURED:
+            if not in_capture:
+                ws[:4].copy_(old[:4], non_blocking=True)
+            if in_capture or key in _WS_CAPTURED:
                 _WS_KEPT.setdefault(key, []).append(old)
                 _WS_CAPTURED.discard(key)
         _WS[key] = ws

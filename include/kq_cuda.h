@@ -326,6 +326,12 @@ int kq_quantized_matmul_chain(const kq_chain_problem *problems, int count, int x
  * synchronises `stream`.  Returns the word (0 = no device-side error). */
 int kq_workspace_error(void *workspace, int clear, void *stream);
 
+/* Sets the calling thread's stream-capture mode (0 global, 1 thread-local, 2 relaxed)
+ * and returns the one before, or -1.  Relaxed for as long as it takes, a workspace
+ * can be allocated and zeroed on another stream while one is captured: as part of
+ * the capture, every replay would wipe what later calls leave in it. */
+int kq_capture_mode(int mode);
+
 /* ---- serving step around the projections ------------------------------------
  * A paged cache holds keys and values of all requests in pages of `page_size`
  * tokens; a request's block table lists its pages.  Slot s is row

@@ -207,3 +207,37 @@ def test_route_stays_in_the_open_groups(cuda, e, groups, scoring):
     rest = [i for i in range(first, e) if i not in left][:k - 4]
     assert all(set(r[:4]) == set(left) and r[4:] == rest for r in idx.tolist())
     assert torch.isfinite(w).all()
+
+
+@pytest.mark.parametrize("call", [lambda f, *a: f(*a), slow], ids=["native", "python"])
+def test_a_workspace_made_in_a_capture_is_none_of_the_graph_s_work(cuda, call):
+    """Two graphs of a stream that no call has used before: either may run first, and
+    neither's replay wipes what the other recorded."""
+    args = attn_inputs(cuda, [(1, 900), (2, 300)], 8, 2, 64, 16, BF)
+    plan = (i32([0], cuda), i32([4], cuda), i32([[-1]], cuda), i32([7], cuda), 4, 4)
+    ref = kq.paged_attention(*args, 2)
+    seq = args[4].clone()
+    s = fresh_stream(cuda)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            if not graphs:
+                call(kq.paged_plan, *plan)  # a small workspace, which the attention outgrows
+            outs.append(call(kq.paged_attention, *args[:4], seq, args[5], 2))
+        graphs.append(g)
+    key = (torch.cuda.current_device(), s.cuda_stream)
+    ws = kq._ext().workspace_peek(*key) if kq._EXT and call is not slow else kq._WS[key]
+    assert not ws.any()
+    with torch.cuda.stream(s):
+        graphs[1].replay()
+        assert torch.equal(outs[1], ref) and call(kq.workspace_error) == 0
+        seq.fill_(10 ** 6)
+        graphs[1].replay()
+        seq.copy_(args[4])
+        graphs[0].replay()
+        assert torch.equal(outs[0], ref)
+        assert call(kq.workspace_error) == 20 and call(kq.workspace_error) == 0
+        graphs[1].replay()
+        assert torch.equal(outs[1], ref) and call(kq.workspace_error) == 0
