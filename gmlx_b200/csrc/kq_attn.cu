@@ -16,8 +16,9 @@
 // by e^(m - m'), two parts (m, l, o) join the same way, and the row is o / l with
 // lse = m + log l.
 // Bound: reading the cache.  64 requests on contexts of up to 16384 (8 kv heads of
-// 128, pages of 16): 1.97 GB in 298 us, 6.6 TB/s, the rate of a plain copy.  One
-// token at a context of 999 is latency: 7.5 us, of which launch, lengths, table and
+// 128, pages of 16): 1.97 GB in 298-306 us, 6.4-6.6 TB/s, the rate of a plain copy
+// (head dim 64 5.4, 256 6.2 TB/s).  One
+// token at a context of 999 is latency: 7.1 us, of which launch, lengths, table and
 // the first keys are a chain of four round trips to memory, the join one more.
 // Above 16 rows the products would bound it (16.8 ms for 4096 tokens on 32768,
 // against 2.0 on the tensor cores).
@@ -31,7 +32,7 @@ namespace {
 
 constexpr int NW = 4, KW = 16, KT = NW * KW;  // warps, keys a warp's step, keys a unit
 constexpr int ROWS = 16;
-constexpr int CTAS = 2;  // blocks an SM
+constexpr int CTAS = 2;  // blocks an SM (of head dim 256 only one fits, 128 KB each: the second half of the grid follows)
 
 template <int D> struct RL {
     static constexpr int STAGES = D >= 256 ? 2 : D >= 128 ? 3 : 6;

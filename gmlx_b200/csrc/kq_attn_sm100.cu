@@ -34,8 +34,9 @@
 // commits take some 500 clocks a step, which the other warp's products cover.
 //
 // 4096 tokens on 32768 cached ones (32 heads over 8, dim 128): 2.05 ms over ten calls,
-// 1.14 PFLOP/s, and 2.42 over thousands, at the power cap (1000 W, 1.44 GHz); a prompt
-// of 512 tokens 20.7 us, of 2400 tokens 69 us.
+// 1.14 PFLOP/s, and 2.4 over thousands, at the power cap (1000 W, 1.44 GHz); 1024 on 8192
+// at head dim 64, 128, 256: 125, 138, 279 us; a prompt of 512 tokens 18.9 us, of 2400
+// tokens 67 us.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -86,9 +87,10 @@ struct Split {
 };
 constexpr int SPLIT_FLOATS = 8 * 256;  // room for one a block in front of the partial rows
 // What a pair costs besides its units, in units: queries, first reference, results.  With 1, 2, 3:
-// a mixed f16 batch of 24 requests 199, 186, 193 us, a prompt of 2400 tokens 80, 69, 70.
+// a mixed f16 batch of 24 requests 199, 186, 193 us, a prompt of 2400 tokens 80, 69, 70 (head
+// dims 64 and 128; not swept at 256).
 constexpr int PAIR_COST = 2;
-constexpr int JOIN_COST = 2;           // what a cut costs, in units: rows written, and the join's launch
+constexpr int JOIN_COST = 2;           // what a cut costs, in units: rows written, and the join's launch (an estimate, not swept)
 
 __device__ __forceinline__ uint64_t gtimer() {
     uint64_t t;

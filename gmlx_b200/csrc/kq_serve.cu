@@ -35,7 +35,7 @@ __device__ __forceinline__ int warp_incl_scan(int v, int lane) {
 // A table entry that this step writes is never read by it (tokens on a new
 // page take its id from the free list), so the blocks need no order.
 // Bound: launch and latency, two dependent rounds of loads and the scan: 64
-// requests of one token 4.0 us, 1000 requests and 44,000 tokens 5.6 us, of which
+// requests of one token 3.9 us, 1000 requests and 44,000 tokens 5.6 us, of which
 // the launch itself is some 2.3.
 constexpr int PLAN_T = 1024;
 
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(ROPE_T) rope_kernel(const RopeArgs a) {
 // are sorted first, so a round looks at one of each lane, and the scores wait in
 // shared memory for the chosen.  Bound: instructions (some 900 a warp with 256
 // experts in 8 groups), at 16 blocks an SM so that 8192 tokens are one wave:
-// 13.3 us; 64 tokens 4.9 us, one token of 128 experts 2.8 us, of which the launch
+// 13.0 us; 64 tokens 4.7 us, one token of 128 experts 2.7 us, of which the launch
 // is 2.3 and the chain load, scores, k rounds the rest.
 
 // Experts of closed groups come behind those of open ones, also behind what a bias of -inf
